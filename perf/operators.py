@@ -55,7 +55,7 @@ def listed():
 
 
 def _log(rng, lo, hi):
-    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 1))))))
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 1)))))))
 
 
 def draw(rng):
