@@ -13,11 +13,14 @@
 
 #include "../../include/k2b.h"
 #include "attention.cuh"
+#include "cross_attention.cuh"
 #include "gemm_w4a4.cuh"
 #include "k2b_common.cuh"
 #include "elementwise.cuh"
 #include "norm_quant.cuh"
+#include "qk_norm_rope.cuh"
 #include "ref_contract.cuh"
+#include "w4_linear.cuh"
 
 #define K2B_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -387,6 +390,132 @@ static int attention_launch(const void* q, const void* k, const void* v, const v
   return launch_status();
 }
 
+// ------------------------------------------- conditioning operators
+// Element types of the conditioning operators (k2_fp8's codes).
+enum CondType : int { COND_FP16 = 1, COND_BF16 = 2 };
+
+static int current_device(int* dev) {
+  cudaError_t e = cudaGetDevice(dev);
+  if (e != cudaSuccess) return (int)e;
+  return *dev < 0 || *dev >= 64 ? (int)cudaErrorInvalidDevice : 0;
+}
+
+template <typename K>
+static int resident_blocks(K kernel, int threads, size_t smem, int* out) {
+  int dev = 0, per_sm = 0, sms = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return (int)e;
+  *out = (per_sm > 0 ? per_sm : 1) * sms;
+  return 0;
+}
+
+// ------------------------------------------------------------ w4_linear
+template <typename T>
+static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void* work, int k, bool rotate,
+                            cudaStream_t st) {
+  const int mblocks = (int)w4_row_blocks(p.m);
+  uint8_t* frag = static_cast<uint8_t*>(work);
+  float* factor = reinterpret_cast<float*>(frag + (long long)mblocks * p.groups * W4_FRAG_BYTES);
+  const long long total = (long long)mblocks * 8 * p.groups;
+  if (total > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  const int pgrid = (int)((total + W4_WARPS - 1) / W4_WARPS);
+  auto prep = rotate ? w4_prepare_kernel<T, true> : w4_prepare_kernel<T, false>;
+  prep<<<pgrid, W4_THREADS, 0, st>>>(static_cast<const T*>(x), x_stride, frag, factor, p.m, p.groups, (int)total);
+  int rc = launch_status();
+  if (rc) return rc;
+  p.frag = frag;
+  p.factor = factor;
+  // warps along k: as many as there are groups for
+  p.kw = p.groups >= 8 ? 8 : p.groups >= 4 ? 4 : p.groups >= 2 ? 2 : 1;
+  // activation blocks per CTA: every block of the rows while they fit the accumulators
+  const int sel = mblocks == 1 ? 0 : mblocks == 2 ? 1 : 2;
+  const int nt = 1 << sel;
+  typedef void (*Kernel)(W4Params);
+  static const Kernel kernels[3] = {w4_linear_kernel<T, 1>, w4_linear_kernel<T, 2>, w4_linear_kernel<T, 4>};
+  static int resident[64][3];
+  int dev = 0;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  if (resident[dev][sel] == 0) {
+    rc = resident_blocks(kernels[sel], W4_THREADS, 0, &resident[dev][sel]);
+    if (rc) return rc;
+  }
+  const int rows_per_cta = 16 * (W4_WARPS / p.kw);
+  const int tiles = (p.n + rows_per_cta - 1) / rows_per_cta;
+  const int gy = (mblocks + nt - 1) / nt;
+  int gx = resident[dev][sel] / gy;
+  gx = gx < 1 ? 1 : gx > tiles ? tiles : gx;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(gx, gy, 1);
+  cfg.blockDim = dim3(W4_THREADS, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernels[sel], p);
+}
+
+// --------------------------------------------------------- qk_norm_rope
+static int qk_norm_rope_launch(QkNormParams p, int dim, int dtype, cudaStream_t st) {
+  const long long items = p.side[0].items + p.side[1].items;
+  const long long grid = (items + QKN_THREADS / 32 - 1) / (QKN_THREADS / 32);
+  if (grid > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  typedef void (*Kernel)(QkNormParams);
+  const Kernel kern = dtype == COND_BF16 ? (dim == 128 ? (Kernel)qk_norm_rope_kernel<__nv_bfloat16, 128>
+                                                       : (Kernel)qk_norm_rope_kernel<__nv_bfloat16, 64>)
+                                         : (dim == 128 ? (Kernel)qk_norm_rope_kernel<__half, 128>
+                                                       : (Kernel)qk_norm_rope_kernel<__half, 64>);
+  kern<<<(unsigned)grid, QKN_THREADS, 0, st>>>(p);
+  return launch_status();
+}
+
+// ------------------------------------------------------ cross attention
+static int cross_few_launch(CrossParams p, int dim, int dtype, cudaStream_t st) {
+  typedef void (*Kernel)(CrossParams);
+  static const Kernel kernels[2][2] = {{cross_few_kernel<__nv_bfloat16, 128>, cross_few_kernel<__nv_bfloat16, 64>},
+                                       {cross_few_kernel<__half, 128>, cross_few_kernel<__half, 64>}};
+  const int ti = dtype == COND_BF16 ? 0 : 1, di = dim == 128 ? 0 : 1;
+  const int smem = di == 0 ? xf_smem_bytes<128>() : xf_smem_bytes<64>();
+  const Kernel kern = kernels[ti][di];
+  static bool attr_set[64][4];
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  if (!attr_set[dev][2 * ti + di]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    attr_set[dev][2 * ti + di] = true;
+  }
+  const long long row_tiles = ((long long)p.group * p.lq + XF_ROWS - 1) / XF_ROWS;
+  const long long ctas = row_tiles * p.kvheads * p.batch;
+  // spread the keys over a cluster while that gives idle SMs work and every warp a tile
+  int splits = 1;
+  while (splits < 8 && ctas * splits * 2 <= 148 && (long long)splits * 2 * XF_WARPS * XF_KEYS <= p.lk) splits *= 2;
+  if (ctas * splits > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  p.row_tiles = (int)row_tiles;
+  p.splits = splits;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)(ctas * splits), 1, 1);
+  cfg.blockDim = dim3(XF_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, kern, p);
+}
+
 // ------------------------------------------------ bounded-wait self-test
 // Exercises the failure path every kernel's waits share (mbar_wait), on a
 // barrier of its own.  One CTA of two warps:
@@ -679,6 +808,88 @@ K2B_EXPORT int k2b_attention_quant(const void* q, const void* k, const void* v, 
                                    long long v_sh, long long v_st, void* stream) {
   return attention_launch(q, k, v, nullptr, nullptr, oq, os, batch, heads, kvheads, lq, lk, dim, q_sb, q_sh, q_st,
                           k_sb, k_sh, k_st, v_sb, v_sh, v_st, 0, (cudaStream_t)stream);
+}
+
+// ------------------------------------------------ conditioning operators
+K2B_EXPORT long long k2b_w4_workspace_bytes(int m, int k) {
+  return m <= 0 || k <= 0 || k % 128 ? -1 : w4_workspace_bytes(m, k);
+}
+
+K2B_EXPORT int k2b_w4_linear(const void* x, long long x_stride, const void* packed, const void* scales,
+                             const void* bias, void* out, void* workspace, int m, int n, int k, int dtype, int rotate,
+                             int act, void* stream) {
+  if (m <= 0 || n <= 0 || k <= 0 || k % 128 || x_stride < (m > 1 ? k : 0) || x_stride % 4 ||
+      (dtype != COND_FP16 && dtype != COND_BF16) || act < W4_NONE || act > W4_SILU)
+    return (int)cudaErrorInvalidValue;
+  if (!x || !packed || !scales || !out || !workspace || reinterpret_cast<uintptr_t>(x) % 8 || !aligned16(packed) ||
+      !aligned16(workspace))
+    return (int)cudaErrorInvalidValue;
+  W4Params p;
+  memset(&p, 0, sizeof(p));
+  p.w = static_cast<const uint8_t*>(packed);
+  p.scales = static_cast<const __half*>(scales);
+  p.bias = bias;
+  p.out = out;
+  p.m = m;
+  p.n = n;
+  p.groups = k / 128;
+  p.act = act;
+  return dtype == COND_BF16 ? w4_linear_launch<__nv_bfloat16>(x, x_stride, p, workspace, k, rotate != 0, (cudaStream_t)stream)
+                            : w4_linear_launch<__half>(x, x_stride, p, workspace, k, rotate != 0, (cudaStream_t)stream);
+}
+
+K2B_EXPORT int k2b_qk_norm_rope(const void* q, const void* k, const void* wq, const void* wk, const void* fq,
+                                const void* fk, void* qo, void* ko, int batch, int lq, int lk, int heads, int kvheads,
+                                int dim, long long q_sb, long long q_sh, long long q_st, long long k_sb,
+                                long long k_sh, long long k_st, int fq_batch, int fk_batch, float eps_q, float eps_k,
+                                int dtype, void* stream) {
+  if (batch <= 0 || lq < 0 || lk < 0 || lq + lk == 0 || heads <= 0 || kvheads <= 0 || (dim != 64 && dim != 128) ||
+      (dtype != COND_FP16 && dtype != COND_BF16) || (fq && fq_batch != 1 && fq_batch != batch) ||
+      (fk && fk_batch != 1 && fk_batch != batch))
+    return (int)cudaErrorInvalidValue;
+  QkNormParams p;
+  p.side[0] = {q, qo, static_cast<const float*>(wq), static_cast<const float*>(fq), q_sb, q_sh, q_st, lq, heads,
+               fq_batch, eps_q, (long long)batch * lq * ((heads + QKN_HEADS - 1) / QKN_HEADS)};
+  p.side[1] = {k, ko, static_cast<const float*>(wk), static_cast<const float*>(fk), k_sb, k_sh, k_st, lk, kvheads,
+               fk_batch, eps_k, (long long)batch * lk * ((kvheads + QKN_HEADS - 1) / QKN_HEADS)};
+  for (const QkNormSide& s : p.side) {
+    if (s.length == 0) continue;
+    if (!s.x || !s.y || !s.w || !aligned16(s.x) || !aligned16(s.y) || !aligned16(s.w) || !aligned16(s.freqs) ||
+        s.sb % 8 || s.sh % 8 || s.st % 8)
+      return (int)cudaErrorInvalidValue;
+  }
+  return qk_norm_rope_launch(p, dim, dtype, (cudaStream_t)stream);
+}
+
+K2B_EXPORT int k2b_cross_attention(const void* q, const void* k, const void* v, const void* lengths, const void* mask,
+                                   const void* bias, void* out, int batch, int heads, int kvheads, int lq, int lk,
+                                   int dim, long long q_sb, long long q_sh, long long q_st, long long k_sb,
+                                   long long k_sh, long long k_st, long long v_sb, long long v_sh, long long v_st,
+                                   long long m_sb, long long m_sh, long long m_sq, long long m_sk, long long bias_sb,
+                                   float scale, int dtype, void* stream) {
+  if (batch <= 0 || heads <= 0 || kvheads <= 0 || heads % kvheads || lq <= 0 || lk < 0 || (dim != 64 && dim != 128) ||
+      (dtype != COND_FP16 && dtype != COND_BF16))
+    return (int)cudaErrorInvalidValue;
+  if (!q || !out || !aligned16(q) || !aligned16(out) ||
+      (lk > 0 && (!k || !v || !aligned16(k) || !aligned16(v))) ||
+      (lengths && reinterpret_cast<uintptr_t>(lengths) % 4) || (bias && reinterpret_cast<uintptr_t>(bias) % 4))
+    return (int)cudaErrorInvalidValue;
+  const long long strides[9] = {q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st};
+  for (long long s : strides)
+    if (s < 0 || s % 8) return (int)cudaErrorInvalidValue;
+  CrossParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = q, p.k = k, p.v = v, p.out = out;
+  p.lengths = static_cast<const int*>(lengths);
+  p.mask = static_cast<const uint8_t*>(mask);
+  p.bias = static_cast<const float*>(bias);
+  p.batch = batch, p.heads = heads, p.kvheads = kvheads, p.group = heads / kvheads, p.lq = lq, p.lk = lk;
+  p.q_sb = q_sb, p.q_sh = q_sh, p.q_st = q_st;
+  p.k_sb = k_sb, p.k_sh = k_sh, p.k_st = k_st;
+  p.v_sb = v_sb, p.v_sh = v_sh, p.v_st = v_st;
+  p.m_sb = m_sb, p.m_sh = m_sh, p.m_sq = m_sq, p.m_sk = m_sk, p.bias_sb = bias_sb;
+  p.scale = scale;
+  return cross_few_launch(p, dim, dtype, (cudaStream_t)stream);
 }
 
 // ---------------------------------------------- e4m3 byte containers

@@ -1,0 +1,251 @@
+// w4_linear.cuh -- a few rows of activations times INT4 weights with group-128
+// scales:
+//
+//   y[r, n] = act( sum_g s[n, g] * sum_{i in g} c[n, i] x'[r, i]  +  b[n] )
+//
+// with c the codes -8..7 of a packed weight (uint8 [N, K/2], low nibble = even
+// column), s its fp16 scales [N, K/128], and x' = x, or x rotated by
+// H128 / sqrt(128) in each group when the weight was (a ConvRot weight).  The
+// activations are not quantised.
+//
+// Bound by the weight bytes, N K / 2: each is used by one row (or a few), and
+// the kernel's whole work is to keep enough of them in flight.
+//
+// w4_prepare_kernel turns the rows into the matrix product's operand:
+// rotated in fp32, scaled by a power of two per (row, group) that brings the
+// group's largest value into [2^14, 2^15), and rounded to fp16.  The rounding
+// is relative to the value for everything within 2^28 of the group's maximum,
+// so it costs a rotated row 2^-12 (a bf16 rounding would cost 2^-9, as much as
+// the output's), and an unrotated bf16 or fp16 row nothing.
+//
+// w4_linear_kernel: a warp takes 16 weight rows (the product's M) and one
+// group of 128 columns at a time, straight from the checkpoint's layout: lane
+// (r, t) loads the 32 codes 32 t.. of rows r and r + 8 with one 16-byte load
+// each.  The k order inside a matrix product is free, so its 8 codes per
+// 32-bit word become two k16 steps without any exchange; x' is laid out for
+// that order by the prepare kernel, one 16-byte load per word.  Codes become
+// fp16 exactly by setting the exponent of 1024 around a nibble.  Each group's
+// sum is scaled by s and the row's power of two in fp32 and added up in fp32.
+#pragma once
+#include "elem16.cuh"
+
+namespace k2b {
+
+constexpr int W4_THREADS = 256;
+constexpr int W4_WARPS = W4_THREADS / 32;
+constexpr int W4_DEPTH = 4;  // groups in flight per warp
+enum W4Act : int { W4_NONE = 0, W4_GELU = 1, W4_SILU = 2 };
+
+// x' of 8 rows and one group: 4 words of 8 columns x 8 rows x 4 column quarters
+constexpr int W4_FRAG_BYTES = 8 * 128 * 2;
+inline long long w4_row_blocks(int m) { return (m + 7) / 8; }
+inline long long w4_workspace_bytes(int m, int k) {
+  return w4_row_blocks(m) * (k / 128) * (W4_FRAG_BYTES + 8 * (long long)sizeof(float));
+}
+
+// One warp per (row, group); rows past m up to a whole block of 8 are zero.
+template <typename T, bool ROTATE>
+__global__ void __launch_bounds__(W4_THREADS)
+    w4_prepare_kernel(const T* x, long long x_stride, uint8_t* frag, float* factor, int m, int groups, int total) {
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int item = blockIdx.x * W4_WARPS + (threadIdx.x >> 5);
+  if (item >= total) return;
+  const int row = item / groups, g = item % groups;
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (row < m) {
+    const uint2 u = __ldg(reinterpret_cast<const uint2*>(x + row * x_stride + g * 128 + lane * 4));
+    const float2 a = Elem16<T>::unpack(u.x), b = Elem16<T>::unpack(u.y);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  }
+  if (ROTATE) {
+    const float a = v[0] + v[1], b = v[0] - v[1], c = v[2] + v[3], d = v[2] - v[3];
+    v[0] = a + c, v[1] = b + d, v[2] = a - c, v[3] = b - d;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, v[i], o);
+        v[i] = (lane & o) ? other - v[i] : v[i] + other;
+      }
+    }
+  }
+  // the largest finite magnitude sets the power of two
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = fabsf(v[i]);
+    if (a <= 3.4028234663852886e38f) top = fmaxf(top, a);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // exponent of 2^(14 - floor(log2 top)), kept inside the normal range
+  int e = 127 + 14 - ((int)(__float_as_uint(top) >> 23) - 127);
+  e = top > 0.0f ? min(max(e, 1), 253) : 127;
+  const float up = __uint_as_float((uint32_t)e << 23), down = __uint_as_float((uint32_t)(254 - e) << 23);
+  uint32_t lo = Elem16<__half>::pack(v[0] * up, v[1] * up), hi = Elem16<__half>::pack(v[2] * up, v[3] * up);
+  // word order (0,4)(1,5)(2,6)(3,7): even lanes hold columns 0..3 of a word, odd lanes 4..7
+  const uint32_t olo = __shfl_xor_sync(0xffffffffu, lo, 1), ohi = __shfl_xor_sync(0xffffffffu, hi, 1);
+  uint2 out;
+  if (lane & 1) {
+    out = make_uint2(__byte_perm(ohi, hi, 0x5410), __byte_perm(ohi, hi, 0x7632));
+  } else {
+    out = make_uint2(__byte_perm(lo, olo, 0x5410), __byte_perm(lo, olo, 0x7632));
+  }
+  const int t = lane >> 3, word = (lane >> 1) & 3;
+  const long long at = ((long long)(row >> 3) * groups + g);
+  *reinterpret_cast<uint2*>(frag + at * W4_FRAG_BYTES + ((word * 8 + (row & 7)) * 4 + t) * 16 + (lane & 1) * 8) = out;
+  // 1/sqrt(128) of the rotation joins the factor
+  if (lane == 0) factor[at * 8 + (row & 7)] = ROTATE ? down * kHadamardScale : down;
+}
+
+// Eight INT4 codes (two's complement nibbles, code i in bits 4i..) -> fp16
+// pairs (0,4) (1,5) (2,6) (3,7).  Nibble ^ 8 is code + 8; under the exponent
+// of 1024 it reads 1024 + (code + 8), and 16 times that for the odd nibbles.
+__device__ __forceinline__ void w4_codes(uint32_t w, uint32_t (&h)[4]) {
+  const __half2 one = __floats2half2_rn(1032.0f, 1032.0f);
+  const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f), off = __floats2half2_rn(-72.0f, -72.0f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t u = i ? w >> 8 : w;
+    const uint32_t a = (u & 0x000F000Fu) ^ 0x64086408u, b = (u & 0x00F000F0u) ^ 0x64806480u;
+    const __half2 ha = __hsub2(*reinterpret_cast<const __half2*>(&a), one);
+    const __half2 hb = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, off);
+    h[2 * i] = *reinterpret_cast<const uint32_t*>(&ha);
+    h[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+  }
+}
+
+__device__ __forceinline__ float w4_act(float y, int act) {
+  if (act == W4_GELU) return 0.5f * y * (1.0f + tanhf(0.7978845608028654f * (y + 0.044715f * y * y * y)));
+  if (act == W4_SILU) return y / (1.0f + expf(-y));
+  return y;
+}
+
+struct W4Params {
+  const uint8_t* w;      // [n, k/2]
+  const __half* scales;  // [n, groups]
+  const uint8_t* frag;   // prepared rows
+  const float* factor;
+  const void* bias;      // [n] or null
+  void* out;             // [m, n]
+  int m, n, groups, act;
+  int kw;                // warps of a CTA along k (1, 2, 4, 8); the others take further rows
+};
+
+// NT: blocks of 8 activation rows of this CTA (blockIdx.y * NT first).
+template <typename T, int NT>
+__global__ void __launch_bounds__(W4_THREADS) w4_linear_kernel(const __grid_constant__ W4Params p) {
+  __shared__ float red[2][W4_WARPS][16][8 * NT + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, t = lane & 3;
+  const int kw = p.kw, rw = W4_WARPS / kw;
+  const int wk = warp % kw, wr = warp / kw;
+  const int tiles = (p.n + 16 * rw - 1) / (16 * rw);
+  const int per_tile = (p.groups + kw - 1) / kw;
+  const long long row_bytes = (long long)p.groups * 64;
+  const int block0 = blockIdx.y * NT;
+  const int mblocks = (p.m + 7) / 8;
+
+  struct Item {
+    uint4 a, b;
+    __half sa, sb;
+  };
+  Item buf[W4_DEPTH];
+  // the next item to load
+  int ltile = blockIdx.x, lj = 0;
+  auto load = [&](Item& it) {
+    const int g = wk + lj * kw;
+    if (ltile < tiles && g < p.groups) {
+      const int n0 = (ltile * rw + wr) * 16 + r;
+      const int ra = min(n0, p.n - 1), rb = min(n0 + 8, p.n - 1);
+      it.a = ldg_stream(p.w + ra * row_bytes + g * 64 + t * 16);
+      it.b = ldg_stream(p.w + rb * row_bytes + g * 64 + t * 16);
+      it.sa = __ldg(p.scales + (long long)ra * p.groups + g);
+      it.sb = __ldg(p.scales + (long long)rb * p.groups + g);
+    }
+    if (++lj == per_tile) {
+      lj = 0;
+      ltile += gridDim.x;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < W4_DEPTH; ++i) load(buf[i]);
+  pdl_wait();
+
+  float acc[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+  int tile = blockIdx.x, j = 0, parity = 0;
+  while (tile < tiles) {
+#pragma unroll
+    for (int s = 0; s < W4_DEPTH; ++s) {
+      if (tile < tiles) {
+        const int g = wk + j * kw;
+        if (g < p.groups) {
+          const uint32_t wa[4] = {buf[s].a.x, buf[s].a.y, buf[s].a.z, buf[s].a.w};
+          const uint32_t wb[4] = {buf[s].b.x, buf[s].b.y, buf[s].b.z, buf[s].b.w};
+          float c[NT][4];
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) c[i][q] = 0.0f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t ha[4], hb[4];
+            w4_codes(wa[w], ha);
+            w4_codes(wb[w], hb);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+              const long long at = (long long)min(block0 + i, mblocks - 1) * p.groups + g;
+              const uint4 xv = *reinterpret_cast<const uint4*>(p.frag + at * W4_FRAG_BYTES + (w * 32 + lane) * 16);
+              mma16816<__half>(c[i], ha[0], hb[0], ha[1], hb[1], xv.x, xv.y);
+              mma16816<__half>(c[i], ha[2], hb[2], ha[3], hb[3], xv.z, xv.w);
+            }
+          }
+          const float sa = __half2float(buf[s].sa), sb = __half2float(buf[s].sb);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const long long at = (long long)min(block0 + i, mblocks - 1) * p.groups + g;
+            const float2 f = *reinterpret_cast<const float2*>(p.factor + at * 8 + 2 * t);
+            acc[i][0] = fmaf(c[i][0] * f.x, sa, acc[i][0]);
+            acc[i][1] = fmaf(c[i][1] * f.y, sa, acc[i][1]);
+            acc[i][2] = fmaf(c[i][2] * f.x, sb, acc[i][2]);
+            acc[i][3] = fmaf(c[i][3] * f.y, sb, acc[i][3]);
+          }
+        }
+        load(buf[s]);
+        if (++j == per_tile) {
+          // the tile's sums over the kw warps, in warp order
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            red[parity][warp][r][8 * i + 2 * t] = acc[i][0];
+            red[parity][warp][r][8 * i + 2 * t + 1] = acc[i][1];
+            red[parity][warp][r + 8][8 * i + 2 * t] = acc[i][2];
+            red[parity][warp][r + 8][8 * i + 2 * t + 1] = acc[i][3];
+            acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+          }
+          __syncthreads();
+          const int cols = 16 * rw;
+          for (int o = threadIdx.x; o < cols * 8 * NT; o += W4_THREADS) {
+            const int nn = o % cols, xr = o / cols;
+            const int n = tile * cols + nn, row = block0 * 8 + xr;
+            if (n < p.n && row < p.m) {
+              float y = 0.0f;
+              for (int q = 0; q < kw; ++q) y += red[parity][(nn >> 4) * kw + q][nn & 15][xr];
+              if (p.bias) y += Elem16<T>::to_float(static_cast<const T*>(p.bias)[n]);
+              static_cast<T*>(p.out)[(long long)row * p.n + n] = Elem16<T>::from_float(w4_act(y, p.act));
+            }
+          }
+          parity ^= 1;
+          j = 0;
+          tile += gridDim.x;
+        }
+      }
+    }
+  }
+}
+
+}  // namespace k2b

@@ -201,6 +201,43 @@ int k2b_attention_quant(const void* q, const void* k, const void* v, void* oq, v
                         long long k_sb, long long k_sh, long long k_st, long long v_sb, long long v_sh,
                         long long v_st, void* stream);
 
+/* ------------------------------------------------ conditioning operators --
+ * A prompt's or an image encoder's states on their way into the DiT stream.
+ * dtype 1 = fp16, 2 = bf16 (activations, bias and outputs); fp32 sums, one
+ * rounding when stored.  No reference counterpart.
+ *
+ * k2b_w4_linear: out [m, n] = act(x' W^T + bias) for a few rows x [m, k] (row
+ * stride x_stride elements, a multiple of 4; x 8-byte aligned), packed INT4
+ * weights u8 [n, k/2] (16-byte aligned) with fp16 scales [n, k/128], k % 128
+ * == 0, bias [n] or null.  rotate: x' = H128/sqrt(128) of x per group of 128
+ * (weights from k2b_rotate_quant), else x' = x.  act 0 none, 1 gelu (tanh
+ * form), 2 silu.  workspace: k2b_w4_workspace_bytes(m, k) bytes (-1 for sizes
+ * it does not take), 16-byte aligned. */
+long long k2b_w4_workspace_bytes(int m, int k);
+int k2b_w4_linear(const void* x, long long x_stride, const void* packed, const void* scales, const void* bias,
+                  void* out, void* workspace, int m, int n, int k, int dtype, int rotate, int act, void* stream);
+/* q [batch, heads, lq, dim], k [batch, kvheads, lk, dim] by element strides
+ * (batch, head, token; multiples of 8, last dim contiguous, dim 64 or 128) ->
+ * qo [batch, lq, heads, dim], ko [batch, lk, kvheads, dim]: per head
+ * R (x rsqrt(mean x^2 + eps) (w + 1)), w fp32 [dim], R from fq / fk fp32
+ * [f_batch (1 or batch), l, dim/2, 2, 2] or none where null.  lk = 0: q alone. */
+int k2b_qk_norm_rope(const void* q, const void* k, const void* wq, const void* wk, const void* fq, const void* fk,
+                     void* qo, void* ko, int batch, int lq, int lk, int heads, int kvheads, int dim, long long q_sb,
+                     long long q_sh, long long q_st, long long k_sb, long long k_sh, long long k_st, int fq_batch,
+                     int fk_batch, float eps_q, float eps_k, int dtype, void* stream);
+/* out [batch, lq, heads*dim] = softmax(q k^T scale + bias) v over the keys that
+ * are not excluded, 0 for a row without any.  Strides as above; k_sb = v_sb = 0
+ * shares K and V among the batch.  Excluded: keys >= lengths[b] (int32 [batch]
+ * or null, clamped to 0..lk), keys with bias -inf (fp32 [batch or 1, lk], batch
+ * stride bias_sb, or null), keys whose mask byte is 0 (by byte strides m_sb,
+ * m_sh, m_sq, m_sk, 0 where broadcast, or null). */
+int k2b_cross_attention(const void* q, const void* k, const void* v, const void* lengths, const void* mask,
+                        const void* bias, void* out, int batch, int heads, int kvheads, int lq, int lk, int dim,
+                        long long q_sb, long long q_sh, long long q_st, long long k_sb, long long k_sh,
+                        long long k_st, long long v_sb, long long v_sh, long long v_st, long long m_sb,
+                        long long m_sh, long long m_sq, long long m_sk, long long bias_sb, float scale, int dtype,
+                        void* stream);
+
 /* ------------------------------------------------ e4m3 byte containers --
  * Forms of the ops above whose INT4 codes travel as e4m3 bytes [rows, K], one
  * byte per code in column order (e4m3 represents -8..7 exactly), instead of
