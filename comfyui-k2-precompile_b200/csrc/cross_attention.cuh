@@ -311,4 +311,642 @@ __global__ void __launch_bounds__(XF_THREADS) cross_few_kernel(const __grid_cons
   if (p.splits > 1) cluster_sync_all();  // the others may still be reading this CTA's sums
 }
 
+// ------------------------------------------------------ tiles of queries
+// Flash attention on tcgen05 for the many-query shapes.  One persistent CTA
+// per SM walks a contiguous range of items; an item is two slots of 128
+// queries that read the same KV head: two heads of an even GQA group at one
+// token tile, or two token tiles of one head (odd groups).  Each K/V tile of
+// 128 keys feeds both slots.
+//
+// TMEM (512 columns): S0 | S1 | O0 | O1 of 128 columns each; P (16-bit)
+// overwrites the first 64 columns of its S.  Products issued by one thread
+// execute in order, so S of the next tile may overwrite P behind the PV
+// product that reads it, and S(j) being complete implies PV(j - 1) is.
+//
+// Warps: 0 TMA loads, 1 products, 2 per-tile side data, 4-7 and 8-11 softmax
+// and output of slot 0 and 1 (a thread owns a row).
+//   - Loads run ahead across items.  While a run of items has the same (b, KV
+//     head) and all its tiles fit the ring, K and V stay where they are: a
+//     short prompt is read once per CTA, not once per query tile.
+//   - Warp 2 turns lengths, bias and key mask into a 128-bit word and 128
+//     addends (log2 units) per tile, and zeroes the V rows of excluded keys
+//     before the product may read them.  A tile with nothing to add and
+//     nothing to exclude takes the path without either.
+//   - A mask that depends on the query or the head is packed to bits by
+//     cross_mask_kernel first (a row then reads 16 bytes per tile instead of
+//     128, and all heads share them); tiles that no row of the item sees are
+//     skipped by every role.
+//   - O is rescaled in TMEM only when a row's maximum grew by more than 2^8
+//     (P and the sum then stay within fp16 and fp32; o = O / l is the same).
+//   - o leaves through shared memory in halves of 64 columns by TMA store,
+//     while the other slot computes.
+constexpr int XT_BM = 128;
+constexpr int XT_BN = 128;
+constexpr int XT_THREADS = 384;
+constexpr int XT_LAUNCH_REGS = 168;  // 65536 / 384; split 80 / 208 by setmaxnreg (128 x 80 + 256 x 208 of 384 x 168)
+constexpr float XT_RESCALE = 8.0f;   // log2 units
+
+template <int D>
+struct XtShape {
+  static constexpr int TILE = 128 * D * 2;            // bytes of a Q, K or V tile
+  static constexpr int STAGES = D == 128 ? 2 : 4;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = OFF_Q + 2 * TILE;
+  static constexpr int OFF_V = OFF_K + STAGES * TILE;
+  static constexpr int OFF_O = OFF_V + STAGES * TILE;  // 2 x 16 KB
+  static constexpr int OFF_AUX = OFF_O + 2 * 16384;
+  static constexpr int AUX = 128 * 4 + 32;             // addends, keep words, flags
+  static constexpr int OFF_BAR = OFF_AUX + STAGES * AUX;
+  static constexpr int NBARS = 4 + 5 * STAGES + 7;
+  static constexpr int SMEM = OFF_BAR + NBARS * 8 + 32 + 1024;
+};
+
+struct CrossMaps {
+  CUtensorMap q, k, v, o;
+};
+
+struct CrossTileParams {
+  CrossParams p;
+  int pairs;            // slot pairs per KV head and token tile
+  int qtiles;           // token tiles (of 128, or 256 where the slots are tiles)
+  int qpair;            // slots are two token tiles of one head
+  int nkt;              // key tiles of lk
+  // packed mask (cross_mask_kernel) or null; row and column words by tile
+  const uint4* bits;    // [mb, mh, mq, nkt]
+  const uint4* cols;    // [mb, mh, ceil(mq / 128), nkt]: keys that some row of 128 sees
+  int mb, mh, mq;       // extents of the packed mask (1 where broadcast)
+};
+
+// Packs a mask that depends on the query or the head: one CTA per 128 rows
+// and 128 keys.
+__global__ void __launch_bounds__(256)
+    cross_mask_kernel(const uint8_t* mask, long long m_sb, long long m_sh, long long m_sq, long long m_sk, int mh,
+                      int mq, int lk, int nkt, uint4* bits, uint4* cols) {
+  pdl_launch_dependents();
+  __shared__ uint32_t any[8][4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kt = blockIdx.x % nkt, qt = blockIdx.x / nkt;
+  const int b = blockIdx.y / mh, h = blockIdx.y % mh;
+  uint32_t seen[4] = {0, 0, 0, 0};
+  const uint8_t* base = mask + b * m_sb + h * m_sh;
+  for (int i = warp; i < 128; i += 8) {
+    const int row = qt * 128 + i;
+    if (row >= mq) break;
+    uint32_t w[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int key = kt * 128 + 32 * c + lane;
+      w[c] = __ballot_sync(0xffffffffu, key < lk && __ldg(base + row * m_sq + key * m_sk) != 0);
+      seen[c] |= w[c];
+    }
+    if (lane == 0) bits[((long long)blockIdx.y * mq + row) * nkt + kt] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (lane < 4) any[warp][lane] = lane == 0 ? seen[0] : lane == 1 ? seen[1] : lane == 2 ? seen[2] : seen[3];
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t a[4] = {0, 0, 0, 0};
+    for (int w = 0; w < 8; ++w)
+      for (int c = 0; c < 4; ++c) a[c] |= any[w][c];
+    cols[((long long)blockIdx.y * ((mq + 127) / 128) + qt) * nkt + kt] = make_uint4(a[0], a[1], a[2], a[3]);
+  }
+}
+
+// Where every role of the CTA is in its range of items.
+struct CrossItem {
+  int b, hk, h0, q0;     // slot t: head h0 + t * hstep, tokens q0 + t * qstep..
+  int n, tiles;          // keys and key tiles of this latent
+  bool resident;         // its K/V tiles stay loaded for the whole run of (b, hk)
+  bool run_first, run_last;
+};
+
+__device__ __forceinline__ CrossItem cross_item(const CrossTileParams& P, int i, int begin, int end, int stages) {
+  const CrossParams& p = P.p;
+  CrossItem it;
+  const int per = P.pairs * P.qtiles;
+  const int key = i / per, rem = i % per;
+  it.b = key / p.kvheads;
+  it.hk = key % p.kvheads;
+  const int pair = rem / P.qtiles, qt = rem % P.qtiles;
+  it.h0 = it.hk * p.group + (P.qpair ? pair : 2 * pair);
+  it.q0 = qt * (P.qpair ? 2 * XT_BM : XT_BM);
+  it.n = p.lengths ? min(max(__ldg(p.lengths + it.b), 0), p.lk) : p.lk;
+  it.tiles = (it.n + XT_BN - 1) / XT_BN;
+  it.resident = !P.bits && it.tiles <= stages;
+  it.run_first = i == begin || rem == 0;
+  it.run_last = i == end - 1 || rem == per - 1;
+  return it;
+}
+
+// The keys of tile j that some row of the item sees (packed mask only).
+__device__ __forceinline__ uint4 cross_seen(const CrossTileParams& P, const CrossItem& it, int j) {
+  uint4 r = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int h = P.mh == 1 ? 0 : it.h0 + (P.qpair ? 0 : t);
+    const int q = P.mq == 1 ? 0 : it.q0 + (P.qpair ? t * XT_BM : 0);
+    if (q >= P.mq) continue;
+    const long long row = ((long long)(P.mb == 1 ? 0 : it.b) * P.mh + h) * ((P.mq + 127) / 128) + q / 128;
+    const uint4 c = P.cols[row * P.nkt + j];
+    r.x |= c.x, r.y |= c.y, r.z |= c.z, r.w |= c.w;
+  }
+  return r;
+}
+
+// The next tile of the item at or after j that has work (tiles if none).
+__device__ __forceinline__ int cross_next_tile(const CrossTileParams& P, const CrossItem& it, int j) {
+  if (P.bits) {
+    while (j < it.tiles) {
+      const uint4 s = cross_seen(P, it, j);
+      if (s.x | s.y | s.z | s.w) break;
+      ++j;
+    }
+  }
+  return j;
+}
+
+__device__ __forceinline__ void named_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(XT_THREADS, 1)
+    cross_tile_kernel(const __grid_constant__ CrossMaps maps, const __grid_constant__ CrossTileParams P) {
+  using X = XtShape<D>;
+  constexpr int NS = X::STAGES;
+  constexpr int HALVES = D / 64;
+  constexpr int BOX = 128 * 128;  // bytes of a 64-column half tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + X::OFF_BAR);
+  uint64_t* q_full = bars;               // [2]
+  uint64_t* q_empty = q_full + 2;        // [2]
+  uint64_t* k_full = q_empty + 2;        // [NS]
+  uint64_t* k_empty = k_full + NS;
+  uint64_t* v_full = k_empty + NS;
+  uint64_t* v_empty = v_full + NS;
+  uint64_t* aux_full = v_empty + NS;
+  uint64_t* s_full = aux_full + NS;      // [2]
+  uint64_t* p_full = s_full + 2;         // [2]
+  uint64_t* o_full = p_full + 2;         // [2]
+  uint64_t* drained = o_full + 2;        // teardown after an abort
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + X::NBARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* range = reinterpret_cast<int*>(tmem_slot + 2);  // [2]
+  const CrossParams& p = P.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&aux_full[i], 1);
+    }
+    mbar_init(drained, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    // Contiguous ranges of equal cost: an item costs its key tiles plus about
+    // two for its queries and output.  (Long batches: equal counts.)
+    const int per = P.pairs * P.qtiles * p.kvheads;
+    const int total = per * p.batch;
+    if (p.lengths && p.batch <= 64) {
+      long long all = 0;
+      for (int b = 0; b < p.batch; ++b) all += (long long)per * ((min(max(__ldg(p.lengths + b), 0), p.lk) + 127) / 128 + 2);
+      const long long at[2] = {all * blockIdx.x / gridDim.x, all * (blockIdx.x + 1) / gridDim.x};
+      long long before = 0;
+      range[0] = range[1] = total;
+      for (int b = 0, e = 0; b < p.batch && e < 2; ++b) {
+        const int cost = (min(max(__ldg(p.lengths + b), 0), p.lk) + 127) / 128 + 2;
+        while (e < 2 && at[e] < before + (long long)per * cost) {
+          range[e] = b * per + (int)((at[e] - before) / cost);
+          ++e;
+        }
+        before += (long long)per * cost;
+      }
+    } else {
+      range[0] = (int)((long long)total * blockIdx.x / gridDim.x);
+      range[1] = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (P.bits) pdl_wait();  // the packed mask
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int begin = range[0], end = range[1];
+  const int hstep = P.qpair ? 0 : 1, qstep = P.qpair ? XT_BM : 0;
+  const bool shared_kv = p.k_sb == 0;
+
+  // what is in flight, for the teardown after an abort
+  int loaded = 0, q_loaded[2] = {0, 0};
+  // (each share is set inside its branch: after a join ptxas would allocate for the smaller one)
+  if (warp >= 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // --------------------------------------------- softmax and output
+    const int t = (warp - 4) >> 2;
+    const int w4 = warp & 3;
+    const int r = 32 * w4 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * w4) << 16);
+    const uint32_t s_col = t * 128, o_col = 256 + t * 128;
+    const float c = p.scale * kLog2e;
+    uint8_t* stage = smem + X::OFF_O + t * 16384;
+    bool ok = true;
+    uint32_t step = 0, out_no = 0;
+    int run_base = 0, next_load = 0;
+    bool stored = false;  // a TMA store may still be reading the staging buffer
+    for (int i = begin; i < end && ok; ++i) {
+      const CrossItem it = cross_item(P, i, begin, end, NS);
+      if (it.resident && it.run_first) run_base = next_load, next_load += it.tiles;
+      const int tok = it.q0 + t * qstep + r, head = it.h0 + t * hstep;
+      const uint4* my_bits = nullptr;
+      if (P.bits) {
+        const long long row = ((long long)(P.mb == 1 ? 0 : it.b) * P.mh + (P.mh == 1 ? 0 : head)) * P.mq +
+                              (P.mq == 1 ? 0 : min(tok, P.mq - 1));
+        my_bits = P.bits + row * P.nkt;
+      }
+      float m_run = -INFINITY, l_run = 0.0f;
+      bool any = false;
+      for (int j = cross_next_tile(P, it, 0); j < it.tiles; j = cross_next_tile(P, it, j + 1)) {
+        const int load = it.resident ? run_base + j : next_load++;
+        const int s = load % NS;
+        uint4 mine = make_uint4(~0u, ~0u, ~0u, ~0u);
+        if (my_bits) mine = my_bits[j];
+        if (!mbar_wait(&aux_full[s], (load / NS) & 1, abort_flag, ERR_WAIT_SOFTMAX) ||
+            !mbar_wait(&s_full[t], step & 1, abort_flag, ERR_WAIT_SOFTMAX)) { ok = false; break; }
+        tc_fence_after();
+        const uint8_t* aux = smem + X::OFF_AUX + s * X::AUX;
+        {
+          const uint4 kw = *reinterpret_cast<const uint4*>(aux + 512);
+          mine.x &= kw.x, mine.y &= kw.y, mine.z &= kw.z, mine.w &= kw.w;
+        }
+        const bool adds = *reinterpret_cast<const int*>(aux + 528) != 0;
+        float sv[128];
+        {
+          uint32_t u[8][16];
+#pragma unroll
+          for (int cc = 0; cc < 8; ++cc) tmem_ld16(lane_base + s_col + 16 * cc, u[cc]);
+#pragma unroll
+          for (int cc = 0; cc < 8; ++cc) {
+            tmem_wait_ld_regs(u[cc]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sv[16 * cc + e] = __uint_as_float(u[cc][e]);
+          }
+        }
+        // scores in log2 units are sv * cm; with addends they are made here and cm is 1
+        float cm = c;
+        if (adds) {
+          cm = 1.0f;
+#pragma unroll
+          for (int e = 0; e < 128; e += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(aux + 4 * e);
+            sv[e] = fmaf(sv[e], c, a.x);
+            sv[e + 1] = fmaf(sv[e + 1], c, a.y);
+            sv[e + 2] = fmaf(sv[e + 2], c, a.z);
+            sv[e + 3] = fmaf(sv[e + 3], c, a.w);
+          }
+        }
+        if (__any_sync(0xffffffffu, (mine.x & mine.y & mine.z & mine.w) != ~0u)) {
+          const uint32_t mw[4] = {mine.x, mine.y, mine.z, mine.w};
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (!((mw[e >> 5] >> (e & 31)) & 1u)) sv[e] = -INFINITY;
+        }
+        float m8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          m8[k] = sv[k];
+#pragma unroll
+          for (int jj = 1; jj < 15; jj += 2) m8[k] = fmax3(m8[k], sv[k + 8 * jj], sv[k + 8 * jj + 8]);
+          m8[k] = fmaxf(m8[k], sv[k + 120]);
+        }
+        const float mx = cm * fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+        // m_run is the reference of P in log2 units (-inf until the row has seen a key)
+        float alpha = 1.0f;
+        bool rescale = false;
+        if (mx > m_run + XT_RESCALE || m_run == -INFINITY) {
+          rescale = m_run != -INFINITY;
+          if (rescale) alpha = exp2_fast(m_run - mx);
+          m_run = mx;
+        }
+        const float base = m_run == -INFINITY ? 0.0f : m_run;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 x = ffma2(make_float2(sv[32 * cc + 2 * e], sv[32 * cc + 2 * e + 1]), make_float2(cm, cm),
+                                   make_float2(-base, -base));
+            const float p0 = exp2_fast(x.x), p1 = exp2_fast(x.y);
+            sum[cc] += p0 + p1;
+            pk[e] = Elem16<T>::pack(p0, p1);
+          }
+          tmem_st16(lane_base + s_col + 16 * cc, pk);
+        }
+        l_run = fmaf(l_run, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+        // O is stable here: S(j) being complete means PV(j - 1) is
+        if (any && __any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+          for (int cc = 0; cc < D / 16; ++cc) {
+            uint32_t u[16];
+            tmem_ld16(lane_base + o_col + 16 * cc, u);
+            tmem_wait_ld_regs(u);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * alpha);
+            tmem_st16(lane_base + o_col + 16 * cc, u);
+          }
+        }
+        any = true;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+        ++step;
+      }
+      if (!ok) break;
+      if (any) {
+        if (!mbar_wait(&o_full[t], out_no & 1, abort_flag, ERR_WAIT_SOFTMAX)) { ok = false; break; }
+        ++out_no;
+        tc_fence_after();
+      }
+      // a row that saw no key is zero (its sum is 0, never NaN)
+      const bool empty = l_run == 0.0f;
+      const float inv = 1.0f / l_run;
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        uint32_t o[32];
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t u[16];
+          if (any) {
+            tmem_ld16(lane_base + o_col + 64 * h + 16 * cc, u);
+            tmem_wait_ld_regs(u);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            o[8 * cc + e] = empty ? 0u : Elem16<T>::pack(__uint_as_float(u[2 * e]) * inv, __uint_as_float(u[2 * e + 1]) * inv);
+        }
+        if (stored && r == 0) bulk_wait_read();
+        named_sync(1 + t);
+        // the 128-byte swizzle of the store's tensor map
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          *reinterpret_cast<uint4*>(stage + r * 128 + ((x ^ (r & 7)) << 4)) =
+              make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        fence_proxy_async_smem();
+        named_sync(1 + t);
+        if (r == 0 && it.q0 + t * qstep < p.lq) {
+          tma_store_4d(&maps.o, stage, 64 * h, it.q0 + t * qstep, head, it.b);
+          bulk_commit();
+        }
+        stored = true;
+      }
+    }
+    if (r == 0) bulk_wait_all();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 0) {
+      // ----------------------------------------------------------- loads
+      if (lane == 0) {
+        bool ok = true;
+        int load = 0, nq = 0;
+        for (int i = begin; i < end && ok; ++i) {
+          const CrossItem it = cross_item(P, i, begin, end, NS);
+          const bool fetch = !it.resident || it.run_first;
+          int j = cross_next_tile(P, it, 0);
+          if (j < it.tiles) {
+#pragma unroll 1
+            for (int t = 0; t < 2 && ok; ++t) {
+              if (nq > 0 && !mbar_wait(&q_empty[t], (nq - 1) & 1, abort_flag, ERR_WAIT_LOAD)) { ok = false; break; }
+              mbar_arrive_expect_tx(&q_full[t], X::TILE);
+              for (int h = 0; h < HALVES; ++h)
+                tma_load_4d(smem + X::OFF_Q + t * X::TILE + h * BOX, &maps.q, &q_full[t], 64 * h, it.q0 + t * qstep,
+                            it.h0 + t * hstep, it.b);
+              q_loaded[t] = nq + 1;
+            }
+            ++nq;
+            for (; j < it.tiles && fetch && ok; j = cross_next_tile(P, it, j + 1)) {
+              const int s = load % NS;
+              const uint32_t ph = (load / NS) & 1;
+              if (load >= NS && !mbar_wait(&k_empty[s], ph ^ 1, abort_flag, ERR_WAIT_LOAD)) { ok = false; break; }
+              mbar_arrive_expect_tx(&k_full[s], X::TILE);
+              for (int h = 0; h < HALVES; ++h)
+                tma_load_4d(smem + X::OFF_K + s * X::TILE + h * BOX, &maps.k, &k_full[s], 64 * h, j * XT_BN, it.hk,
+                            shared_kv ? 0 : it.b);
+              loaded = 2 * load + 1;
+              if (load >= NS && !mbar_wait(&v_empty[s], ph ^ 1, abort_flag, ERR_WAIT_LOAD)) { ok = false; break; }
+              mbar_arrive_expect_tx(&v_full[s], X::TILE);
+              for (int h = 0; h < HALVES; ++h)
+                tma_load_4d(smem + X::OFF_V + s * X::TILE + h * BOX, &maps.v, &v_full[s], 64 * h, j * XT_BN, it.hk,
+                            shared_kv ? 0 : it.b);
+              loaded = 2 * load + 2;
+              ++load;
+            }
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // -------------------------------------------------------- products
+      if (lane == 0) {
+        constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0 : 1;
+        constexpr uint32_t idesc_s = make_idesc(1, fmt, fmt, 0, 0, XT_BM, XT_BN);  // Q K^T, both K-major
+        constexpr uint32_t idesc_o = make_idesc(1, fmt, fmt, 0, 1, XT_BM, D);      // P V, V MN-major
+        // One step: tile j of item i, its ring slot `load`.
+        struct Step {
+          int i, j, load, item_no;
+          bool first, last, release;
+        };
+        CrossItem it;
+        int run_base = 0, next_load = 0, item_no = -1;
+        auto open_item = [&](Step& st) {  // first step at or after item st.i
+          for (; st.i < end; ++st.i) {
+            it = cross_item(P, st.i, begin, end, NS);
+            const int j = cross_next_tile(P, it, 0);
+            if (it.resident && it.run_first) run_base = next_load, next_load += it.tiles;
+            if (j >= it.tiles) continue;
+            ++item_no;
+            st.j = j;
+            st.first = true;
+            st.item_no = item_no;
+            return true;
+          }
+          return false;
+        };
+        auto close_step = [&](Step& st) {  // ring slot, whether it is the item's last, whether it frees the slot
+          st.load = it.resident ? run_base + st.j : next_load++;
+          st.last = cross_next_tile(P, it, st.j + 1) >= it.tiles;
+          st.release = !it.resident || it.run_last;
+        };
+        auto advance = [&](Step& st) {
+          if (!st.last) {
+            st.j = cross_next_tile(P, it, st.j + 1);
+            st.first = false;
+          } else {
+            ++st.i;
+            if (!open_item(st)) return false;
+          }
+          close_step(st);
+          return true;
+        };
+        auto issue_s = [&](int t, const Step& st) {
+          const int s = st.load % NS;
+          // 16 columns further: 32 B on within a 64-column half, BOX on to the next (descriptors count 16 B)
+          const uint64_t qa = umma_desc_sw128(smem_u32(smem + X::OFF_Q + t * X::TILE), 16, 1024);
+          const uint64_t ka = umma_desc_sw128(smem_u32(smem + X::OFF_K + s * X::TILE), 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+            mma_bf16_ss(tmem + t * 128, qa + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          mma_commit(&s_full[t]);
+          if (st.last) mma_commit(&q_empty[t]);
+          if (t == 1 && st.release) mma_commit(&k_empty[s]);
+        };
+        Step cur;
+        cur.i = begin;
+        bool have = open_item(cur);
+        if (have) close_step(cur);
+        bool ok = have;
+        if (ok) ok = mbar_wait(&k_full[cur.load % NS], (cur.load / NS) & 1, abort_flag, ERR_WAIT_MMA);
+#pragma unroll 1
+        for (int t = 0; t < 2 && ok; ++t) {
+          ok = mbar_wait(&q_full[t], 0, abort_flag, ERR_WAIT_MMA);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(t, cur);
+        }
+        for (uint32_t step = 0; have && ok; ++step) {
+          Step nxt = cur;
+          const bool more = advance(nxt);
+          const int s = cur.load % NS;
+          const uint32_t ph = (cur.load / NS) & 1;
+#pragma unroll 1
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (t == 0 && !(mbar_wait(&v_full[s], ph, abort_flag, ERR_WAIT_MMA) &&
+                            mbar_wait(&aux_full[s], ph, abort_flag, ERR_WAIT_MMA))) { ok = false; break; }
+            if (!mbar_wait(&p_full[t], step & 1, abort_flag, ERR_WAIT_MMA)) { ok = false; break; }
+            tc_fence_after();
+            // 16 keys further: 16 rows of 128 B; the two 64-column halves are BOX apart (LBO)
+            const uint64_t va = umma_desc_sw128(smem_u32(smem + X::OFF_V + s * X::TILE), BOX, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              mma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, va + kk * (2048 >> 4), idesc_o,
+                          (!cur.first || kk > 0) ? 1u : 0u);
+            if (cur.last) mma_commit(&o_full[t]);
+            if (t == 1 && cur.release) mma_commit(&v_empty[s]);
+            if (more) {
+              if (t == 0 && !mbar_wait(&k_full[nxt.load % NS], (nxt.load / NS) & 1, abort_flag, ERR_WAIT_MMA)) { ok = false; break; }
+              if (nxt.first && !mbar_wait(&q_full[t], nxt.item_no & 1, abort_flag, ERR_WAIT_MMA)) { ok = false; break; }
+              tc_fence_after();
+              issue_s(t, nxt);
+            }
+          }
+          cur = nxt;
+          have = more;
+        }
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------- side data of every K/V load
+      bool ok = true;
+      int load = 0;
+      for (int i = begin; i < end && ok; ++i) {
+        const CrossItem it = cross_item(P, i, begin, end, NS);
+        if (it.resident && !it.run_first) continue;
+        const bool key_mask = p.mask && !P.bits;
+        for (int j = cross_next_tile(P, it, 0); j < it.tiles; j = cross_next_tile(P, it, j + 1)) {
+          const int s = load % NS;
+          float add[4];
+          uint32_t word[4];
+          bool plain = true;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int key = j * XT_BN + 32 * c + lane;
+            bool keep = key < it.n;
+            add[c] = 0.0f;
+            if (keep && p.bias) {
+              const float raw = __ldg(p.bias + it.b * p.bias_sb + key);
+              keep = raw != -INFINITY;
+              // log2 units; a finite addend stays finite
+              add[c] = raw * kLog2e;
+              if (fabsf(raw) <= 3.4028234663852886e38f) add[c] = fminf(fmaxf(add[c], -3.4028234663852886e38f), 3.4028234663852886e38f);
+              if (!keep) add[c] = 0.0f;
+            }
+            if (keep && key_mask) keep = __ldg(p.mask + it.b * p.m_sb + key * p.m_sk) != 0;
+            word[c] = __ballot_sync(0xffffffffu, keep);
+            plain = plain && !__any_sync(0xffffffffu, add[c] != 0.0f);
+          }
+          uint4 live = make_uint4(word[0], word[1], word[2], word[3]);
+          if (P.bits) {
+            const uint4 seen = cross_seen(P, it, j);
+            live.x &= seen.x, live.y &= seen.y, live.z &= seen.z, live.w &= seen.w;
+          }
+          if (!mbar_wait(&v_full[s], (load / NS) & 1, abort_flag, ERR_WAIT_LOAD)) { ok = false; break; }
+          uint8_t* aux = smem + X::OFF_AUX + s * X::AUX;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) reinterpret_cast<float*>(aux)[32 * c + lane] = add[c];
+          if (lane == 0) {
+            *reinterpret_cast<uint4*>(aux + 512) = make_uint4(word[0], word[1], word[2], word[3]);
+            *reinterpret_cast<int*>(aux + 528) = plain ? 0 : 1;
+          }
+          // V rows of keys that nobody sees
+          const uint32_t lw[4] = {live.x, live.y, live.z, live.w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (!((lw[c] >> lane) & 1u)) {
+              uint8_t* row = smem + X::OFF_V + s * X::TILE + (32 * c + lane) * 128;
+#pragma unroll
+              for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+                for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(row + h * BOX + 16 * x) = make_uint4(0, 0, 0, 0);
+            }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&aux_full[s]);
+          ++load;
+        }
+      }
+    }
+  }
+
+  // ------------------------------------------------------------ teardown
+  if (*abort_flag) {
+    if (warp == 0 && lane == 0) {
+      for (int t = 0; t < 2; ++t)
+        if (q_loaded[t]) mbar_drain(&q_full[t], (q_loaded[t] - 1) & 1);
+      const int kl = (loaded + 1) / 2, vl = loaded / 2;
+      for (int x = max(0, kl - NS); x < kl; ++x) mbar_drain(&k_full[x % NS], (x / NS) & 1);
+      for (int x = max(0, vl - NS); x < vl; ++x) mbar_drain(&v_full[x % NS], (x / NS) & 1);
+    }
+    if (warp == 1 && lane == 0) {  // behind every product issued
+      mma_commit(drained);
+      mbar_drain(drained, 0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 }  // namespace k2b

@@ -64,15 +64,16 @@ static int make_map_2d(CUtensorMap* map, CUtensorMapDataType dt, size_t esize, c
 
 // 4-D map (d, token, head, batch) over a strided bf16 [B, H, L, D] view.
 static int make_map_4d_bf16(CUtensorMap* map, const void* base, uint64_t D, uint64_t L, uint64_t H, uint64_t B,
-                            uint64_t s_tok, uint64_t s_head, uint64_t s_batch, uint32_t box_d, uint32_t box_tok) {
+                            uint64_t s_tok, uint64_t s_head, uint64_t s_batch, uint32_t box_d, uint32_t box_tok,
+                            CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return (int)cudaErrorInitializationError;
   cuuint64_t dims[4] = {D, L, H, B};
   cuuint64_t strides[3] = {s_tok * 2, s_head * 2, s_batch * 2};
   cuuint32_t box[4] = {box_d, box_tok, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  CUresult r = enc(map, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
@@ -516,6 +517,107 @@ static int cross_few_launch(CrossParams p, int dim, int dtype, cudaStream_t st) 
   return (int)cudaLaunchKernelEx(&cfg, kern, p);
 }
 
+// Which kernel takes the call: tiles of 128 queries from XT_MIN_QUERIES on.
+// Below, most rows of a tile would be empty.  A negative or zero scale and
+// axes with stride 0 (other than a shared batch of K and V) also take the
+// other kernel: the tile kernel's row maximum is that of q k^T, and a tensor
+// map has no stride 0.
+constexpr int XT_MIN_QUERIES = 33;
+static bool cross_takes_tiles(const CrossParams& p) {
+  return p.lq >= XT_MIN_QUERIES && p.lk > 0 && p.scale > 0.0f && p.q_sb > 0 && p.q_sh > 0 && p.q_st > 0 && p.k_sh > 0 &&
+         p.k_st > 0 && p.v_sh > 0 && p.v_st > 0 && (p.k_sb == 0) == (p.v_sb == 0);
+}
+
+struct MaskExtent {
+  int mb, mh, mq, nkt;
+  long long bits_bytes, bytes;
+};
+// The packed form of a mask that depends on the query or the head (bytes = 0: not needed).
+static MaskExtent cross_mask_extent(const CrossParams& p) {
+  MaskExtent e;
+  memset(&e, 0, sizeof(e));
+  e.nkt = (p.lk + XT_BN - 1) / XT_BN;
+  if (!p.mask || (p.m_sh == 0 && p.m_sq == 0)) return e;
+  e.mb = p.m_sb ? p.batch : 1;
+  e.mh = p.m_sh ? p.heads : 1;
+  e.mq = p.m_sq ? p.lq : 1;
+  const long long planes = (long long)e.mb * e.mh * e.nkt * (long long)sizeof(uint4);
+  e.bits_bytes = planes * e.mq;
+  e.bytes = e.bits_bytes + planes * ((e.mq + 127) / 128);
+  return e;
+}
+
+static int cross_tile_launch(const CrossParams& p, void* work, int dim, int dtype, cudaStream_t st) {
+  const CUtensorMapDataType dt = dtype == COND_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CrossMaps maps;
+  const uint64_t B = p.batch, H = p.heads, Hk = p.kvheads, D = dim;
+  const bool shared = p.k_sb == 0;
+  int rc = make_map_4d_bf16(&maps.q, p.q, D, p.lq, H, B, p.q_st, p.q_sh, p.q_sb, 64, XT_BM, dt);
+  if (!rc) rc = make_map_4d_bf16(&maps.k, p.k, D, p.lk, Hk, shared ? 1 : B, p.k_st, p.k_sh, shared ? D : p.k_sb, 64, XT_BN, dt);
+  if (!rc) rc = make_map_4d_bf16(&maps.v, p.v, D, p.lk, Hk, shared ? 1 : B, p.v_st, p.v_sh, shared ? D : p.v_sb, 64, XT_BN, dt);
+  if (!rc) rc = make_map_4d_bf16(&maps.o, p.out, D, p.lq, H, B, H * D, D, (uint64_t)p.lq * H * D, 64, XT_BM, dt);
+  if (rc) return rc;
+  CrossTileParams P;
+  memset(&P, 0, sizeof(P));
+  P.p = p;
+  P.qpair = p.group % 2;  // an odd group cannot pair two heads on one KV head
+  P.pairs = P.qpair ? p.group : p.group / 2;
+  const int span = P.qpair ? 2 * XT_BM : XT_BM;
+  P.qtiles = (p.lq + span - 1) / span;
+  const MaskExtent e = cross_mask_extent(p);
+  P.nkt = e.nkt;
+  const long long items = (long long)P.pairs * P.qtiles * p.kvheads * p.batch;
+  if (items > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  if (e.bytes) {
+    const long long gx = (long long)e.nkt * ((e.mq + 127) / 128), gy = (long long)e.mb * e.mh;
+    if (!work || !aligned16(work) || gx > 0x7fffffffLL || gy > 65535) return (int)cudaErrorInvalidValue;
+    P.mb = e.mb, P.mh = e.mh, P.mq = e.mq;
+    uint4* bits = static_cast<uint4*>(work);
+    uint4* cols = reinterpret_cast<uint4*>(static_cast<uint8_t*>(work) + e.bits_bytes);
+    P.bits = bits;
+    P.cols = cols;
+    cross_mask_kernel<<<dim3((unsigned)gx, (unsigned)gy), 256, 0, st>>>(p.mask, p.m_sb, p.m_sh, p.m_sq, p.m_sk, e.mh,
+                                                                      e.mq, p.lk, e.nkt, bits, cols);
+    rc = launch_status();
+    if (rc) return rc;
+  }
+  typedef void (*Kernel)(CrossMaps, CrossTileParams);
+  static const Kernel kernels[2][2] = {{cross_tile_kernel<__nv_bfloat16, 128>, cross_tile_kernel<__nv_bfloat16, 64>},
+                                       {cross_tile_kernel<__half, 128>, cross_tile_kernel<__half, 64>}};
+  const int ti = dtype == COND_BF16 ? 0 : 1, di = dim == 128 ? 0 : 1;
+  const int smem = di == 0 ? XtShape<128>::SMEM : XtShape<64>::SMEM;
+  const Kernel kern = kernels[ti][di];
+  static int sms[64];
+  static bool attr_set[64][4];
+  int dev = 0;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  if (!attr_set[dev][2 * ti + di]) {
+    cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err != cudaSuccess) return (int)err;
+    // setmaxnreg splits exactly the registers the CTA is launched with: any
+    // other allocation could leave a warpgroup waiting for registers.
+    cudaFuncAttributes fa;
+    err = cudaFuncGetAttributes(&fa, kern);
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    if (err != cudaSuccess) return (int)err;
+    if (fa.numRegs != XT_LAUNCH_REGS) return (int)cudaErrorInvalidConfiguration;
+    attr_set[dev][2 * ti + di] = true;
+  }
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)(items < sms[dev] ? items : sms[dev]), 1, 1);
+  cfg.blockDim = dim3(XT_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = e.bytes ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, kern, maps, P);
+}
+
 // ------------------------------------------------ bounded-wait self-test
 // Exercises the failure path every kernel's waits share (mbar_wait), on a
 // barrier of its own.  One CTA of two warps:
@@ -861,8 +963,20 @@ K2B_EXPORT int k2b_qk_norm_rope(const void* q, const void* k, const void* wq, co
   return qk_norm_rope_launch(p, dim, dtype, (cudaStream_t)stream);
 }
 
+K2B_EXPORT long long k2b_cross_workspace_bytes(int batch, int heads, int lq, int lk, long long m_sb, long long m_sh,
+                                               long long m_sq) {
+  if (batch <= 0 || heads <= 0 || lq <= 0 || lk < 0) return -1;
+  CrossParams p;
+  memset(&p, 0, sizeof(p));
+  static const uint8_t some = 0;
+  p.mask = &some;
+  p.batch = batch, p.heads = heads, p.lq = lq, p.lk = lk;
+  p.m_sb = m_sb, p.m_sh = m_sh, p.m_sq = m_sq;
+  return lq >= XT_MIN_QUERIES ? cross_mask_extent(p).bytes : 0;
+}
+
 K2B_EXPORT int k2b_cross_attention(const void* q, const void* k, const void* v, const void* lengths, const void* mask,
-                                   const void* bias, void* out, int batch, int heads, int kvheads, int lq, int lk,
+                                   const void* bias, void* out, void* workspace, int batch, int heads, int kvheads, int lq, int lk,
                                    int dim, long long q_sb, long long q_sh, long long q_st, long long k_sb,
                                    long long k_sh, long long k_st, long long v_sb, long long v_sh, long long v_st,
                                    long long m_sb, long long m_sh, long long m_sq, long long m_sk, long long bias_sb,
@@ -889,7 +1003,8 @@ K2B_EXPORT int k2b_cross_attention(const void* q, const void* k, const void* v, 
   p.v_sb = v_sb, p.v_sh = v_sh, p.v_st = v_st;
   p.m_sb = m_sb, p.m_sh = m_sh, p.m_sq = m_sq, p.m_sk = m_sk, p.bias_sb = bias_sb;
   p.scale = scale;
-  return cross_few_launch(p, dim, dtype, (cudaStream_t)stream);
+  return cross_takes_tiles(p) ? cross_tile_launch(p, workspace, dim, dtype, (cudaStream_t)stream)
+                              : cross_few_launch(p, dim, dtype, (cudaStream_t)stream);
 }
 
 // ---------------------------------------------- e4m3 byte containers

@@ -785,10 +785,15 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, length
     out = torch.empty((B, Lq, H * D), dtype=q.dtype, device=q.device)
     if out.numel() == 0:
         return out
-    check(lib().k2b_cross_attention(
+    L = lib()
+    work = None
+    if ms[1] or ms[2]:  # depends on the head or the query: packed to bits first
+        nbytes = L.k2b_cross_workspace_bytes(B, H, Lq, Lk, *ms[:3])
+        work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    check(L.k2b_cross_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), None if lengths is None else lengths.data_ptr(),
-        None if mask is None else mask.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), B, H,
-        Hk, Lq, Lk, D, *qs, *ks, *vs, *ms, bs, D ** -0.5 if scale is None else scale, code, _stream()),
+        None if mask is None else mask.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
+        None if work is None else work.data_ptr(), B, H, Hk, Lq, Lk, D, *qs, *ks, *vs, *ms, bs, D ** -0.5 if scale is None else scale, code, _stream()),
         "k2b_cross_attention")
     return out
 

@@ -230,9 +230,13 @@ int k2b_qk_norm_rope(const void* q, const void* k, const void* wq, const void* w
  * shares K and V among the batch.  Excluded: keys >= lengths[b] (int32 [batch]
  * or null, clamped to 0..lk), keys with bias -inf (fp32 [batch or 1, lk], batch
  * stride bias_sb, or null), keys whose mask byte is 0 (by byte strides m_sb,
- * m_sh, m_sq, m_sk, 0 where broadcast, or null). */
+ * m_sh, m_sq, m_sk, 0 where broadcast, or null).  workspace: the packed form of
+ * a mask with m_sh or m_sq, k2b_cross_workspace_bytes bytes on a 16-byte
+ * boundary (0 bytes: may be null). */
+long long k2b_cross_workspace_bytes(int batch, int heads, int lq, int lk, long long m_sb, long long m_sh,
+                                    long long m_sq);
 int k2b_cross_attention(const void* q, const void* k, const void* v, const void* lengths, const void* mask,
-                        const void* bias, void* out, int batch, int heads, int kvheads, int lq, int lk, int dim,
+                        const void* bias, void* out, void* workspace, int batch, int heads, int kvheads, int lq, int lk, int dim,
                         long long q_sb, long long q_sh, long long q_st, long long k_sb, long long k_sh,
                         long long k_st, long long v_sb, long long v_sh, long long v_st, long long m_sb,
                         long long m_sh, long long m_sq, long long m_sk, long long bias_sb, float scale, int dtype,

@@ -109,6 +109,6 @@ def test_c_entries_refuse(lib):
         q, None, P, None, P, None, P, None, 2, lq, 0, heads, 1, dim, 64, 64, st, 0, 0, 0, fb, 1, 1e-6, 1e-6, dtype, None)
     assert {qk(q=None), qk(lq=0), qk(heads=0), qk(dim=32), qk(st=4), qk(fb=3), qk(dtype=0), qk(q=odd)} == {1}
     ca = lambda q=P, k=P, heads=2, hk=1, lq=1, lk=4, dim=64, st=64, dtype=2: lib.k2b_cross_attention(  # noqa: E731
-        q, k, P, None, None, None, P, 1, heads, hk, lq, lk, dim, *([64] * 8), st, 0, 0, 0, 0, 0, 1.0, dtype, None)
+        q, k, P, None, None, None, P, None, 1, heads, hk, lq, lk, dim, *([64] * 8), st, 0, 0, 0, 0, 0, 1.0, dtype, None)
     assert {ca(q=None), ca(k=None), ca(heads=3, hk=2), ca(lq=0), ca(lk=-1), ca(dim=96), ca(st=12), ca(st=-8),
             ca(dtype=0), ca(q=odd)} == {1}
