@@ -1,4 +1,5 @@
-"""ctypes binding of libk2b (include/k2b.h).
+"""ctypes binding of libk2b (include/k2b.h), and the native binding of the
+conditioning operators (csrc/torch_bind.cpp) on top of it.
 
 The library is the only compute path: if it is missing or fails to load, every
 op raises.  There is no eager / PyTorch / CPU fallback.
@@ -10,6 +11,7 @@ import os
 import threading
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libk2b.so")
+BIND_PATH = os.path.join(os.path.dirname(LIB_PATH), "_bind.so")
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -93,11 +95,25 @@ SIGNATURES = {
 }
 
 _lib = None
+_bind = None
 _lock = threading.Lock()
 
 
 class K2BError(RuntimeError):
     """A libk2b entry point returned a non-zero status."""
+
+
+def _build() -> None:
+    """Build both libraries if this is a source tree without them."""
+    build_py = os.path.join(os.path.dirname(os.path.dirname(LIB_PATH)), "..", "build.py")
+    if not os.path.exists(build_py):
+        raise K2BError(f"libk2b not built: {LIB_PATH} is missing")
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("_k2b_build", build_py)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.build()
 
 
 def lib() -> ctypes.CDLL:
@@ -106,15 +122,7 @@ def lib() -> ctypes.CDLL:
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):
-                build_py = os.path.join(os.path.dirname(os.path.dirname(LIB_PATH)), "..", "build.py")
-                if not os.path.exists(build_py):
-                    raise K2BError(f"libk2b not built: {LIB_PATH} is missing")
-                import importlib.util
-
-                spec = importlib.util.spec_from_file_location("_k2b_build", build_py)
-                mod = importlib.util.module_from_spec(spec)
-                spec.loader.exec_module(mod)
-                mod.build()
+                _build()
             L = ctypes.CDLL(LIB_PATH)
             for name, (res, args) in SIGNATURES.items():
                 fn = getattr(L, name)
@@ -122,6 +130,26 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = L
     return _lib
+
+
+def bind():
+    """The native binding of the conditioning operators (a module), loaded on
+    first use."""
+    global _bind
+    if _bind is None:
+        lib()
+        with _lock:
+            if _bind is None:
+                if not os.path.exists(BIND_PATH):
+                    _build()
+                import importlib.machinery
+                import importlib.util
+
+                loader = importlib.machinery.ExtensionFileLoader("_bind", BIND_PATH)
+                mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_bind", loader))
+                loader.exec_module(mod)
+                _bind = mod
+    return _bind
 
 
 def check(rc: int, what: str) -> None:

@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._native import K2BError, check, lib
+from ._native import K2BError, bind, check, lib
 
 GROUP = 128
 HEAD_DIM = 128
@@ -594,26 +594,10 @@ def attention_quant_e4m3(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
 # few rows against 4-bit weights, head norms with the rotation, and attention
 # to a sequence of another length.  bf16 and fp16; forward only, like every
 # op here.
+# The checks, allocations and launches are native (csrc/torch_bind.cpp): at
+# these sizes the host side of a call is most of its time.
 
-_DTYPE = {torch.float16: 1, torch.bfloat16: 2}
 _ACT = {"none": 0, "gelu": 1, "silu": 2}
-
-
-def _dtype_code(t: torch.Tensor, what: str) -> int:
-    code = _DTYPE.get(t.dtype)
-    if code is None:
-        raise ValueError(f"{what}: bf16 or fp16 expected, got {t.dtype}")
-    return code
-
-
-def _on_device(dev: torch.device, what: str, *ts: Optional[torch.Tensor]) -> None:
-    """Every tensor on ``dev``, and ``dev`` the current device (whose stream
-    the op launches on)."""
-    for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: all tensors on one CUDA device expected, got {t.device} and {dev}")
-    if dev.type != "cuda" or dev.index != torch.cuda.current_device():
-        raise ValueError(f"{what}: tensors on {dev}, which is not the current CUDA device")
 
 
 def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -629,69 +613,8 @@ def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, bias:
     summed in fp32 and rounded once.  Meant for up to about a hundred rows (a
     modulation vector, a prompt's states): every 32 rows read the weight
     again; above that quantise the activations and use ``gemm_bf16``."""
-    code = _dtype_code(x, "w4_linear: x")
-    if packed.dtype != torch.uint8 or scales.dtype != torch.float16 or packed.dim() != 2:
-        raise ValueError("w4_linear: packed uint8 [n, k/2] and fp16 scales expected")
-    n, k = packed.shape[0], 2 * packed.shape[1]
-    if k == 0 or k % GROUP or x.dim() == 0 or x.shape[-1] != k or tuple(scales.shape) != (n, k // GROUP):
-        raise ValueError(f"w4_linear: x {tuple(x.shape)}, packed {tuple(packed.shape)} and scales "
-                         f"{tuple(scales.shape)} do not fit (k a multiple of 128)")
-    if act not in _ACT:
-        raise ValueError(f"w4_linear: act {act!r} is none of {', '.join(_ACT)}")
-    if not packed.is_contiguous() or not scales.is_contiguous():
-        raise ValueError("w4_linear: contiguous packed and scales expected")
-    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
-        raise ValueError("w4_linear: bias [n] in x's dtype expected")
-    _on_device(x.device, "w4_linear", packed, scales, bias)
-    lead = x.shape[:-1]
-    m = x.numel() // k
-    out = torch.empty((*lead, n), dtype=x.dtype, device=x.device)
-    if m == 0 or n == 0:
-        return out
-    if x.is_contiguous():
-        stride = k
-    else:
-        try:
-            rows = x.view(m, k)
-        except RuntimeError:
-            rows = None
-        if rows is None or rows.stride(1) != 1 or (m > 1 and rows.stride(0) < k):
-            raise ValueError("w4_linear: the rows of x must have one stride and contiguous columns")
-        stride = rows.stride(0)
-    if stride % 4 or x.data_ptr() % 8:
-        raise ValueError("w4_linear: x's rows must start on 8-byte boundaries")
-    if packed.data_ptr() % 16:
-        raise ValueError("w4_linear: packed must start on a 16-byte boundary")
-    L = lib()
-    work = torch.empty(L.k2b_w4_workspace_bytes(m, k), dtype=torch.uint8, device=x.device)
-    check(L.k2b_w4_linear(x.data_ptr(), stride, packed.data_ptr(), scales.data_ptr(),
-                          None if bias is None else bias.data_ptr(), out.data_ptr(), work.data_ptr(), m, n, k, code,
-                          1 if rotate else 0, _ACT[act], _stream()), "k2b_w4_linear")
-    return out
-
-
-def _heads(t: torch.Tensor, name: str):
-    """(B, H, L, D) and the strides of a 16-bit [B, H, L, D] view whose heads
-    are contiguous and start on 16-byte boundaries."""
-    if t.dim() != 4 or t.shape[3] not in (64, 128):
-        raise ValueError(f"{name}: [B, H, L, D] with D 64 or 128 expected, got {tuple(t.shape)}")
-    shape, (sb, sh, st, sd) = t.shape, t.stride()
-    # the stride of an axis with one entry says nothing
-    st = st if shape[2] > 1 else shape[3]
-    sh = sh if shape[1] > 1 else shape[3]
-    sb = sb if shape[0] > 1 else shape[3]
-    if t.numel() and (sd != 1 or sb % 8 or sh % 8 or st % 8 or t.data_ptr() % 16):
-        raise ValueError(f"{name}: contiguous heads on 16-byte boundaries expected (strides {t.stride()})")
-    return shape, (sb, sh, st)
-
-
-def _rope_batch(f: Optional[torch.Tensor], B: int, L: int, D: int, name: str) -> int:
-    if f is None:
-        return 1
-    per = L * D * 2
-    if f.dtype != torch.float32 or not f.is_contiguous() or f.data_ptr() % 16 or f.numel() not in (per, B * per):
-        raise ValueError(f"qk_norm_rope: {name} must be contiguous fp32 [L, D/2, 2, 2] (or with a leading B)")
-    return 1 if f.numel() == per else B
+    _need(act in _ACT, f"w4_linear: act {act!r} is none of {', '.join(_ACT)}")
+    return bind().w4_linear(x, packed, scales, bias, rotate, _ACT[act])
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], wq: torch.Tensor, wk: Optional[torch.Tensor],
@@ -707,34 +630,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], wq: torch.Tensor, w
     carry no position.  k = None norms the queries alone (keys kept from an
     earlier step).  fp32 throughout, rounded once.  Returns (q', k') as
     [B, H, L, D] views of token-major memory, which the attention ops take."""
-    code = _dtype_code(q, "qk_norm_rope: q")
-    (B, H, Lq, D), qs = _heads(q, "qk_norm_rope: q")
-    if wq.dtype != torch.float32 or wq.numel() != D or not wq.is_contiguous() or wq.data_ptr() % 16:
-        raise ValueError("qk_norm_rope: wq fp32 [D] expected")
-    fqb = _rope_batch(freqs_q, B, Lq, D, "freqs_q")
-    qo = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
-    Hk, Lk, ks, fkb, ko = 1, 0, (0, 0, 0), 1, None
-    if k is None:
-        if wk is not None or freqs_k is not None:
-            raise ValueError("qk_norm_rope: wk and freqs_k go with k")
-    else:
-        (Bk, Hk, Lk, Dk), ks = _heads(k, "qk_norm_rope: k")
-        if Bk != B or Dk != D or k.dtype != q.dtype:
-            raise ValueError(f"qk_norm_rope: k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
-        if wk is None or wk.dtype != torch.float32 or wk.numel() != D or not wk.is_contiguous() or wk.data_ptr() % 16:
-            raise ValueError("qk_norm_rope: wk fp32 [D] expected")
-        fkb = _rope_batch(freqs_k, B, Lk, D, "freqs_k")
-        ko = torch.empty((B, Lk, Hk, D), dtype=q.dtype, device=q.device)
-    _on_device(q.device, "qk_norm_rope", k, wq, wk, freqs_q, freqs_k)
-    if H == 0 or Hk == 0:
-        raise ValueError("qk_norm_rope: no heads")
-    if B * (Lq + Lk):
-        check(lib().k2b_qk_norm_rope(
-            q.data_ptr(), None if k is None else k.data_ptr(), wq.data_ptr(), None if wk is None else wk.data_ptr(),
-            None if freqs_q is None else freqs_q.data_ptr(), None if freqs_k is None else freqs_k.data_ptr(),
-            qo.data_ptr(), None if ko is None else ko.data_ptr(), B, Lq, Lk, H, Hk, D, *qs, *ks, fqb, fkb, eps_q,
-            eps_k, code, _stream()), "k2b_qk_norm_rope")
-    return qo.transpose(1, 2), None if ko is None else ko.transpose(1, 2)
+    return bind().qk_norm_rope(q, k, wq, wk, freqs_q, freqs_k, eps_q, eps_k)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Optional[torch.Tensor] = None,
@@ -754,48 +650,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, length
     K may hold anything at a key that is left out, and V too unless a mask
     shows that key to other queries.  scale: 1/sqrt(D) by default.  Returns
     [B, Lq, H*D] in q's dtype."""
-    code = _dtype_code(q, "cross_attention: q")
-    (B, H, Lq, D), qs = _heads(q, "cross_attention: q")
-    (Bk, Hk, Lk, Dk), ks = _heads(k, "cross_attention: k")
-    _, vs = _heads(v, "cross_attention: v")
-    if k.shape != v.shape or Dk != D or Bk not in (1, B) or Hk == 0 or H % Hk or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"cross_attention: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype} and v "
-                         f"{tuple(v.shape)} {v.dtype} do not go together")
-    if Bk != B:
-        ks, vs = (0, ks[1], ks[2]), (0, vs[1], vs[2])
-    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or
-                                not lengths.is_contiguous()):
-        raise ValueError("cross_attention: lengths int32 [B] expected")
-    ms = (0, 0, 0, 0)
-    if mask is not None:
-        shape = tuple(mask.shape)
-        if mask.dtype != torch.bool or len(shape) not in (2, 4) or shape[-1] != Lk or shape[0] not in (1, B) or \
-                (len(shape) == 4 and (shape[1] not in (1, H) or shape[2] not in (1, Lq))):
-            raise ValueError(f"cross_attention: mask bool [B|1, H|1, Lq|1, Lk] or [B|1, Lk] expected, got "
-                             f"{mask.dtype} {shape}")
-        st = [s if z != 1 else 0 for s, z in zip(mask.stride()[:-1], shape)]
-        ms = (st[0], st[1], st[2], mask.stride(3)) if len(shape) == 4 else (st[0], 0, 0, mask.stride(1))
-    bs = 0
-    if bias is not None:
-        if bias.dtype != torch.float32 or bias.dim() != 2 or bias.shape[0] not in (1, B) or bias.shape[1] != Lk or \
-                (Lk > 1 and bias.stride(1) != 1):
-            raise ValueError("cross_attention: bias fp32 [B|1, Lk] with contiguous keys expected")
-        bs = bias.stride(0) if bias.shape[0] != 1 else 0
-    _on_device(q.device, "cross_attention", k, v, lengths, mask, bias)
-    out = torch.empty((B, Lq, H * D), dtype=q.dtype, device=q.device)
-    if out.numel() == 0:
-        return out
-    L = lib()
-    work = None
-    if ms[1] or ms[2]:  # depends on the head or the query: packed to bits first
-        nbytes = L.k2b_cross_workspace_bytes(B, H, Lq, Lk, *ms[:3])
-        work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    check(L.k2b_cross_attention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), None if lengths is None else lengths.data_ptr(),
-        None if mask is None else mask.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
-        None if work is None else work.data_ptr(), B, H, Hk, Lq, Lk, D, *qs, *ks, *vs, *ms, bs, D ** -0.5 if scale is None else scale, code, _stream()),
-        "k2b_cross_attention")
-    return out
+    return bind().cross_attention(q, k, v, lengths, mask, bias, scale)
 
 
 def device_error(reset: bool = True) -> int:

@@ -23,7 +23,7 @@ def w4_args(**change):
     (dict(packed=torch.zeros(8, 128, dtype=torch.int8)), "uint8"),
     (dict(packed=torch.zeros(8, 96, dtype=torch.uint8)), "do not fit"),
     (dict(packed=torch.zeros(128, 8, dtype=torch.uint8).t()), "contiguous"),
-    (dict(scales=torch.zeros(8, 2)), "fp16 scales"),
+    (dict(scales=torch.zeros(8, 2)), "fp16 scales expected"),
     (dict(scales=torch.zeros(8, 3, dtype=torch.float16)), "do not fit"),
     (dict(bias=torch.zeros(7, dtype=BF)), "bias"),
     (dict(bias=torch.zeros(8)), "bias"),
