@@ -323,8 +323,15 @@ __global__ void __launch_bounds__(XF_THREADS) cross_few_kernel(const __grid_cons
 // execute in order, so S of the next tile may overwrite P behind the PV
 // product that reads it, and S(j) being complete implies PV(j - 1) is.
 //
-// Warps: 0 TMA loads, 1 products, 2 per-tile side data, 4-7 and 8-11 softmax
-// and output of slot 0 and 1 (a thread owns a row).
+// Warps: 0 TMA loads, 1 products, 2 per-tile side data, 3 the walk, 4-7 and
+// 8-11 softmax and output of slot 0 and 1 (a thread owns a row).
+//   - Warp 3 alone decides what is next: it writes one record per step (item,
+//     key tile, ring slot, what to load and free) into a ring that the other
+//     roles read, so that no division, length or mask lookup stands between a
+//     barrier and the product behind it.
+//   - Warp 1 runs as a whole warp with one elected lane issuing: descriptors
+//     are then in uniform registers.  Issued from a one-lane branch, each
+//     product cost 80-100 cycles of scalar work against 64 of tensor time.
 //   - Loads run ahead across items.  While a run of items has the same (b, KV
 //     head) and all its tiles fit the ring, K and V stay where they are: a
 //     short prompt is read once per CTA, not once per query tile.
@@ -338,13 +345,20 @@ __global__ void __launch_bounds__(XF_THREADS) cross_few_kernel(const __grid_cons
 //     skipped by every role.
 //   - O is rescaled in TMEM only when a row's maximum grew by more than 2^8
 //     (P and the sum then stay within fp16 and fp32; o = O / l is the same).
-//   - o leaves through shared memory in halves of 64 columns by TMA store,
-//     while the other slot computes.
+//   - Part of the exponentials run on the FMA pipe (exp2_poly): at 128 x 128
+//     scores per 1024 cycles of tensor time the MUFU alone would take as long
+//     as the products do.
 constexpr int XT_BM = 128;
 constexpr int XT_BN = 128;
 constexpr int XT_THREADS = 384;
 constexpr int XT_LAUNCH_REGS = 168;  // 65536 / 384; split 80 / 208 by setmaxnreg (128 x 80 + 256 x 208 of 384 x 168)
 constexpr float XT_RESCALE = 8.0f;   // log2 units
+constexpr int XT_RECORDS = 8;        // steps the walk may be ahead of the slowest role
+constexpr int XT_READERS = 11;       // loads, products, side data, eight softmax warps
+constexpr int XT_POLY_PAIRS = 6;     // of the 16 pairs of a 32-key chunk, those that exp2_poly takes
+__host__ __device__ constexpr bool xt_poly_pair(int e) {  // spread evenly over the chunk
+  return (e + 1) * XT_POLY_PAIRS / 16 != e * XT_POLY_PAIRS / 16;
+}
 
 template <int D>
 struct XtShape {
@@ -353,16 +367,16 @@ struct XtShape {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + 2 * TILE;
   static constexpr int OFF_V = OFF_K + STAGES * TILE;
-  static constexpr int OFF_O = OFF_V + STAGES * TILE;  // 2 x 16 KB
-  static constexpr int OFF_AUX = OFF_O + 2 * 16384;
+  static constexpr int OFF_AUX = OFF_V + STAGES * TILE;
   static constexpr int AUX = 128 * 4 + 32;             // addends, keep words, flags
-  static constexpr int OFF_BAR = OFF_AUX + STAGES * AUX;
-  static constexpr int NBARS = 4 + 5 * STAGES + 7;
+  static constexpr int OFF_REC = OFF_AUX + STAGES * AUX;
+  static constexpr int OFF_BAR = OFF_REC + XT_RECORDS * 32;
+  static constexpr int NBARS = 4 + 5 * STAGES + 7 + 2 * XT_RECORDS;
   static constexpr int SMEM = OFF_BAR + NBARS * 8 + 32 + 1024;
 };
 
 struct CrossMaps {
-  CUtensorMap q, k, v, o;
+  CUtensorMap q, k, v;
 };
 
 struct CrossTileParams {
@@ -411,69 +425,177 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Where every role of the CTA is in its range of items.
-struct CrossItem {
-  int b, hk, h0, q0;     // slot t: head h0 + t * hstep, tokens q0 + t * qstep..
-  int n, tiles;          // keys and key tiles of this latent
-  bool resident;         // its K/V tiles stay loaded for the whole run of (b, hk)
-  bool run_first, run_last;
+// One step of the walk: key tile j of an item, or an item without any.
+enum CrossFlags : int {
+  XS_FIRST = 1,     // first tile of its item
+  XS_LAST = 2,      // last tile of its item (also set for an item without tiles)
+  XS_EMPTY = 4,     // no key: the output is zero and nothing else happens
+  XS_LOAD = 8,      // K and V are loaded for this step (else they are still there)
+  XS_FREE = 16,     // the ring slot is free after this step
+  XS_END = 32,
+};
+struct CrossStep {
+  int flags, j, load, item_no;  // load: running number of the K/V load (ring slot load % STAGES)
+  int b, hk, h0, q0;            // slot t: head h0 + t * hstep, tokens q0 + t * qstep..
 };
 
-__device__ __forceinline__ CrossItem cross_item(const CrossTileParams& P, int i, int begin, int end, int stages) {
-  const CrossParams& p = P.p;
-  CrossItem it;
-  const int per = P.pairs * P.qtiles;
-  const int key = i / per, rem = i % per;
-  it.b = key / p.kvheads;
-  it.hk = key % p.kvheads;
-  const int pair = rem / P.qtiles, qt = rem % P.qtiles;
-  it.h0 = it.hk * p.group + (P.qpair ? pair : 2 * pair);
-  it.q0 = qt * (P.qpair ? 2 * XT_BM : XT_BM);
-  it.n = p.lengths ? min(max(__ldg(p.lengths + it.b), 0), p.lk) : p.lk;
-  it.tiles = (it.n + XT_BN - 1) / XT_BN;
-  it.resident = !P.bits && it.tiles <= stages;
-  it.run_first = i == begin || rem == 0;
-  it.run_last = i == end - 1 || rem == per - 1;
-  return it;
-}
-
 // The keys of tile j that some row of the item sees (packed mask only).
-__device__ __forceinline__ uint4 cross_seen(const CrossTileParams& P, const CrossItem& it, int j) {
+__device__ __forceinline__ uint4 cross_seen(const CrossTileParams& P, int b, int h0, int q0, int j) {
   uint4 r = make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int h = P.mh == 1 ? 0 : it.h0 + (P.qpair ? 0 : t);
-    const int q = P.mq == 1 ? 0 : it.q0 + (P.qpair ? t * XT_BM : 0);
+    const int h = P.mh == 1 ? 0 : h0 + (P.qpair ? 0 : t);
+    const int q = P.mq == 1 ? 0 : q0 + (P.qpair ? t * XT_BM : 0);
     if (q >= P.mq) continue;
-    const long long row = ((long long)(P.mb == 1 ? 0 : it.b) * P.mh + h) * ((P.mq + 127) / 128) + q / 128;
+    const long long row = ((long long)(P.mb == 1 ? 0 : b) * P.mh + h) * ((P.mq + 127) / 128) + q / 128;
     const uint4 c = P.cols[row * P.nkt + j];
     r.x |= c.x, r.y |= c.y, r.z |= c.z, r.w |= c.w;
   }
   return r;
 }
 
-// The next tile of the item at or after j that has work (tiles if none).
-__device__ __forceinline__ int cross_next_tile(const CrossTileParams& P, const CrossItem& it, int j) {
-  if (P.bits) {
-    while (j < it.tiles) {
-      const uint4 s = cross_seen(P, it, j);
-      if (s.x | s.y | s.z | s.w) break;
-      ++j;
-    }
-  }
-  return j;
+__device__ __forceinline__ int cross_keys(const CrossParams& p, int b) {
+  return p.lengths ? min(max(__ldg(p.lengths + b), 0), p.lk) : p.lk;
 }
 
-__device__ __forceinline__ void named_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+// This CTA's items [range[0], range[1]): contiguous ranges of equal cost, an
+// item costing its key tiles plus about two for its queries and output.
+// (More than 64 latents: equal counts.)
+__device__ __forceinline__ void cross_range(const CrossTileParams& P, int (&range)[2]) {
+  const CrossParams& p = P.p;
+  const int per = P.pairs * P.qtiles * p.kvheads;
+  const int total = per * p.batch;
+  if (!p.lengths || p.batch > 64) {
+    range[0] = (int)((long long)total * blockIdx.x / gridDim.x);
+    range[1] = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
+    return;
+  }
+  long long all = 0;
+  for (int b = 0; b < p.batch; ++b) all += (long long)per * ((cross_keys(p, b) + XT_BN - 1) / XT_BN + 2);
+  const long long at[2] = {all * blockIdx.x / gridDim.x, all * (blockIdx.x + 1) / gridDim.x};
+  long long before = 0;
+  range[0] = range[1] = total;
+  int e = 0;
+  for (int b = 0; b < p.batch && e < 2; ++b) {
+    const int cost = (cross_keys(p, b) + XT_BN - 1) / XT_BN + 2;
+    while (e < 2 && at[e] < before + (long long)per * cost) {
+      range[e] = b * per + (int)((at[e] - before) / cost);
+      ++e;
+    }
+    before += (long long)per * cost;
+  }
+}
 
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int x, int y, int z, int w) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
-               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes;
+}
+__device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// 32 bytes, a whole sector per lane.
+__device__ __forceinline__ void st_global_32b(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tadd.rn.f32x2 rd, ra, "
+      "rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+// The larger of the two or three, NaN if any is.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 64 columns of this lane's row, complete on return.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, "
+      "%34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, "
+      "%54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      :
+        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st64(uint32_t taddr, const uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13"
+      ", %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33"
+      ", %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53"
+      ", %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64};"
+      ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(r[32]), "r"(r[33]), "r"(r[34]), "r"(r[35]),
+        "r"(r[36]), "r"(r[37]), "r"(r[38]), "r"(r[39]), "r"(r[40]), "r"(r[41]), "r"(r[42]), "r"(r[43]), "r"(r[44]),
+        "r"(r[45]), "r"(r[46]), "r"(r[47]), "r"(r[48]), "r"(r[49]), "r"(r[50]), "r"(r[51]), "r"(r[52]), "r"(r[53]),
+        "r"(r[54]), "r"(r[55]), "r"(r[56]), "r"(r[57]), "r"(r[58]), "r"(r[59]), "r"(r[60]), "r"(r[61]), "r"(r[62]),
+        "r"(r[63])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13"
+      ", %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// 2^x of a pair on the FMA pipe, x at most about 2^7 and not NaN: x = n + f
+// with n the nearest integer (adding 1.5 * 2^23 rounds to it and leaves it in
+// the low bits), 2^f by a minimax polynomial on [-1/2, 1/2] with constant
+// term 1 (fitted for relative error: 1.0e-4 in degree 3, 2.8e-6 in degree 4),
+// n added to the exponent field.  x is cut at -127, where the result is 0
+// exactly, so an excluded key (-inf) adds nothing.  P is rounded to 2^-9
+// (bf16) or 2^-12 (fp16) afterwards, so degree 3 and 4 lose nothing to it.
+template <int DEGREE>
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  static_assert(DEGREE == 3 || DEGREE == 4, "fitted degrees");
+  constexpr float c1 = DEGREE == 3 ? 0.6932829022407532f : 0.6931241750717163f;
+  constexpr float c2 = DEGREE == 3 ? 0.24221095442771912f : 0.24024099111557007f;
+  constexpr float c3 = DEGREE == 3 ? 0.05500892922282219f : 0.055906426161527634f;
+  constexpr float c4 = 0.009582852944731712f;
+  x.x = fmaxf(x.x, -127.0f);
+  x.y = fmaxf(x.y, -127.0f);
+  const float2 y = fadd2(x, make_float2(kRoundMagic, kRoundMagic));
+  // -n as a product: the packed forms have no negation
+  const float2 f = fadd2(x, ffma2(y, make_float2(-1.0f, -1.0f), make_float2(kRoundMagic, kRoundMagic)));
+  float2 r = make_float2(c3, c3);
+  if (DEGREE == 4) r = ffma2(make_float2(c4, c4), f, r);
+  r = ffma2(r, f, make_float2(c2, c2));
+  r = ffma2(r, f, make_float2(c1, c1));
+  r = ffma2(r, f, make_float2(1.0f, 1.0f));
+  return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(y.x) << 23)),
+                     __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(y.y) << 23)));
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(XT_THREADS, 1)
@@ -482,6 +604,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
   constexpr int NS = X::STAGES;
   constexpr int HALVES = D / 64;
   constexpr int BOX = 128 * 128;  // bytes of a 64-column half tile
+  constexpr bool F16 = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + X::OFF_BAR);
@@ -495,12 +618,16 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
   uint64_t* s_full = aux_full + NS;      // [2]
   uint64_t* p_full = s_full + 2;         // [2]
   uint64_t* o_full = p_full + 2;         // [2]
-  uint64_t* drained = o_full + 2;        // teardown after an abort
+  uint64_t* rec_full = o_full + 2;       // [XT_RECORDS]
+  uint64_t* rec_empty = rec_full + XT_RECORDS;
+  uint64_t* drained = rec_empty + XT_RECORDS;  // teardown after an abort
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + X::NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* range = reinterpret_cast<int*>(tmem_slot + 2);  // [2]
+  int4* records = reinterpret_cast<int4*>(smem + X::OFF_REC);  // two per step
+  const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
   const CrossParams& p = P.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const bool leader = elect_lane() != 0;  // products are ordered only within one thread
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -517,31 +644,13 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
       mbar_init(&v_empty[i], 1);
       mbar_init(&aux_full[i], 1);
     }
+    for (int i = 0; i < XT_RECORDS; ++i) {
+      mbar_init(&rec_full[i], 1);
+      mbar_init(&rec_empty[i], XT_READERS);
+    }
     mbar_init(drained, 1);
     *abort_flag = 0;
     fence_barrier_init();
-    // Contiguous ranges of equal cost: an item costs its key tiles plus about
-    // two for its queries and output.  (Long batches: equal counts.)
-    const int per = P.pairs * P.qtiles * p.kvheads;
-    const int total = per * p.batch;
-    if (p.lengths && p.batch <= 64) {
-      long long all = 0;
-      for (int b = 0; b < p.batch; ++b) all += (long long)per * ((min(max(__ldg(p.lengths + b), 0), p.lk) + 127) / 128 + 2);
-      const long long at[2] = {all * blockIdx.x / gridDim.x, all * (blockIdx.x + 1) / gridDim.x};
-      long long before = 0;
-      range[0] = range[1] = total;
-      for (int b = 0, e = 0; b < p.batch && e < 2; ++b) {
-        const int cost = (min(max(__ldg(p.lengths + b), 0), p.lk) + 127) / 128 + 2;
-        while (e < 2 && at[e] < before + (long long)per * cost) {
-          range[e] = b * per + (int)((at[e] - before) / cost);
-          ++e;
-        }
-        before += (long long)per * cost;
-      }
-    } else {
-      range[0] = (int)((long long)total * blockIdx.x / gridDim.x);
-      range[1] = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
-    }
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -552,13 +661,29 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int begin = range[0], end = range[1];
   const int hstep = P.qpair ? 0 : 1, qstep = P.qpair ? XT_BM : 0;
-  const bool shared_kv = p.k_sb == 0;
+
+  // Record `no` of the walk, by a whole warp, and whether there is one (ok:
+  // the wait for it).  Its place is free for the walk once every reader has it
+  // in registers.
+  // (the softmax warps wait inline: a call would cost them their registers)
+  auto rec_ready = [&](uint32_t no) {
+    return mbar_wait_fast(smem_u32(&rec_full[no % XT_RECORDS]), (no / XT_RECORDS) & 1, abort_addr, ERR_WAIT_LOAD);
+  };
+  auto read_step = [&](uint32_t no, CrossStep& st, bool ok) {
+    const uint32_t at = no % XT_RECORDS;
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    const int4 u = records[2 * at], v = records[2 * at + 1];
+    st.flags = u.x, st.j = u.y, st.load = u.z, st.item_no = u.w;
+    st.b = v.x, st.hk = v.y, st.h0 = v.z, st.q0 = v.w;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&rec_empty[at]);
+    return (st.flags & XS_END) == 0;
+  };
 
   // what is in flight, for the teardown after an abort
-  int loaded = 0, q_loaded[2] = {0, 0};
-  // (each share is set inside its branch: after a join ptxas would allocate for the smaller one)
+  int k_loads = 0, v_loads = 0, q_loads[2] = {0, 0};
+  // (each share of the registers is set inside its branch: after a join ptxas would allocate for the smaller one)
   if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // --------------------------------------------- softmax and output
@@ -568,104 +693,115 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
     const uint32_t lane_base = tmem + ((uint32_t)(32 * w4) << 16);
     const uint32_t s_col = t * 128, o_col = 256 + t * 128;
     const float c = p.scale * kLog2e;
-    uint8_t* stage = smem + X::OFF_O + t * 16384;
-    bool ok = true;
     uint32_t step = 0, out_no = 0;
-    int run_base = 0, next_load = 0;
-    bool stored = false;  // a TMA store may still be reading the staging buffer
-    for (int i = begin; i < end && ok; ++i) {
-      const CrossItem it = cross_item(P, i, begin, end, NS);
-      if (it.resident && it.run_first) run_base = next_load, next_load += it.tiles;
-      const int tok = it.q0 + t * qstep + r, head = it.h0 + t * hstep;
-      const uint4* my_bits = nullptr;
-      if (P.bits) {
-        const long long row = ((long long)(P.mb == 1 ? 0 : it.b) * P.mh + (P.mh == 1 ? 0 : head)) * P.mq +
-                              (P.mq == 1 ? 0 : min(tok, P.mq - 1));
-        my_bits = P.bits + row * P.nkt;
+    float m_run = -INFINITY, l_run = 0.0f;
+    CrossStep st;
+    for (uint32_t no = 0;
+         read_step(no, st, mbar_wait_s(smem_u32(&rec_full[no % XT_RECORDS]), (no / XT_RECORDS) & 1, abort_addr, ERR_WAIT_SOFTMAX));
+         ++no) {
+      const int tok = st.q0 + t * qstep + r, head = st.h0 + t * hstep;
+      const bool first = st.flags & XS_FIRST;
+      if (first) {
+        m_run = -INFINITY;
+        l_run = 0.0f;
       }
-      float m_run = -INFINITY, l_run = 0.0f;
-      bool any = false;
-      for (int j = cross_next_tile(P, it, 0); j < it.tiles; j = cross_next_tile(P, it, j + 1)) {
-        const int load = it.resident ? run_base + j : next_load++;
-        const int s = load % NS;
+      if (!(st.flags & XS_EMPTY)) {
+        const int s = st.load % NS;
         uint4 mine = make_uint4(~0u, ~0u, ~0u, ~0u);
-        if (my_bits) mine = my_bits[j];
-        if (!mbar_wait(&aux_full[s], (load / NS) & 1, abort_flag, ERR_WAIT_SOFTMAX) ||
-            !mbar_wait(&s_full[t], step & 1, abort_flag, ERR_WAIT_SOFTMAX)) { ok = false; break; }
+        if (P.bits) {
+          const long long row = ((long long)(P.mb == 1 ? 0 : st.b) * P.mh + (P.mh == 1 ? 0 : head)) * P.mq +
+                                (P.mq == 1 ? 0 : min(tok, P.mq - 1));
+          mine = P.bits[row * P.nkt + st.j];
+        }
+        if (!mbar_wait_s(smem_u32(&aux_full[s]), (st.load / NS) & 1, abort_addr, ERR_WAIT_SOFTMAX) ||
+            !mbar_wait_s(smem_u32(&s_full[t]), step & 1, abort_addr, ERR_WAIT_SOFTMAX)) break;
+        ++step;
         tc_fence_after();
+        // The loops below stay rolled, 64 columns a turn: the whole row in
+        // registers makes 90 KB of code, and the kernel then waits for
+        // instructions (hit rate of the SM's instruction cache 74%).
         const uint8_t* aux = smem + X::OFF_AUX + s * X::AUX;
         {
           const uint4 kw = *reinterpret_cast<const uint4*>(aux + 512);
           mine.x &= kw.x, mine.y &= kw.y, mine.z &= kw.z, mine.w &= kw.w;
         }
         const bool adds = *reinterpret_cast<const int*>(aux + 528) != 0;
-        float sv[128];
-        {
-          uint32_t u[8][16];
+        const bool cuts = __any_sync(0xffffffffu, (mine.x & mine.y & mine.z & mine.w) != ~0u);
+        // first pass: the row's maximum; with addends or excluded keys S is
+        // replaced by the scores in log2 units (sv * cm with cm = 1)
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t u[64];
+          tmem_ld64(lane_base + s_col + 64 * half, u);
+          if (adds) {
 #pragma unroll
-          for (int cc = 0; cc < 8; ++cc) tmem_ld16(lane_base + s_col + 16 * cc, u[cc]);
-#pragma unroll
-          for (int cc = 0; cc < 8; ++cc) {
-            tmem_wait_ld_regs(u[cc]);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sv[16 * cc + e] = __uint_as_float(u[cc][e]);
+            for (int e = 0; e < 64; e += 4) {
+              const float4 a = *reinterpret_cast<const float4*>(aux + 4 * (64 * half + e));
+              u[e] = __float_as_uint(fmaf(__uint_as_float(u[e]), c, a.x));
+              u[e + 1] = __float_as_uint(fmaf(__uint_as_float(u[e + 1]), c, a.y));
+              u[e + 2] = __float_as_uint(fmaf(__uint_as_float(u[e + 2]), c, a.z));
+              u[e + 3] = __float_as_uint(fmaf(__uint_as_float(u[e + 3]), c, a.w));
+            }
           }
-        }
-        // scores in log2 units are sv * cm; with addends they are made here and cm is 1
-        float cm = c;
-        if (adds) {
-          cm = 1.0f;
+          if (cuts) {
+            const uint32_t lo = half ? mine.z : mine.x, hi = half ? mine.w : mine.y;
 #pragma unroll
-          for (int e = 0; e < 128; e += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(aux + 4 * e);
-            sv[e] = fmaf(sv[e], c, a.x);
-            sv[e + 1] = fmaf(sv[e + 1], c, a.y);
-            sv[e + 2] = fmaf(sv[e + 2], c, a.z);
-            sv[e + 3] = fmaf(sv[e + 3], c, a.w);
+            for (int e = 0; e < 64; ++e)
+              if (!(((e < 32 ? lo : hi) >> (e & 31)) & 1u)) u[e] = 0xff800000u;  // -inf
           }
-        }
-        if (__any_sync(0xffffffffu, (mine.x & mine.y & mine.z & mine.w) != ~0u)) {
-          const uint32_t mw[4] = {mine.x, mine.y, mine.z, mine.w};
+          if (adds || cuts) tmem_st64(lane_base + s_col + 64 * half, u);
+          float m4[4];
 #pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (!((mw[e >> 5] >> (e & 31)) & 1u)) sv[e] = -INFINITY;
-        }
-        float m8[8];
+          for (int k = 0; k < 4; ++k) {
+            m4[k] = __uint_as_float(u[k]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          m8[k] = sv[k];
-#pragma unroll
-          for (int jj = 1; jj < 15; jj += 2) m8[k] = fmax3(m8[k], sv[k + 8 * jj], sv[k + 8 * jj + 8]);
-          m8[k] = fmaxf(m8[k], sv[k + 120]);
+            for (int jj = 1; jj < 15; jj += 2)
+              m4[k] = fmax3_nan(m4[k], __uint_as_float(u[k + 4 * jj]), __uint_as_float(u[k + 4 * jj + 4]));
+            m4[k] = fmax_nan(m4[k], __uint_as_float(u[k + 60]));
+          }
+          mx = fmax3_nan(mx, fmax_nan(m4[0], m4[1]), fmax_nan(m4[2], m4[3]));
         }
-        const float mx = cm * fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
-        // m_run is the reference of P in log2 units (-inf until the row has seen a key)
+        if (adds || cuts) tmem_wait_st();
+        const float cm = adds ? 1.0f : c;
+        mx *= cm;
+        // m_run is the reference of P in log2 units: -inf until the row has
+        // seen a key, NaN once a score was NaN or +inf (then the row is NaN)
         float alpha = 1.0f;
         bool rescale = false;
-        if (mx > m_run + XT_RESCALE || m_run == -INFINITY) {
+        if (mx > m_run + XT_RESCALE || m_run == -INFINITY || mx != mx) {
+          const float next = mx == INFINITY ? __int_as_float(0x7fc00000) : mx;
           rescale = m_run != -INFINITY;
-          if (rescale) alpha = exp2_fast(m_run - mx);
-          m_run = mx;
+          if (rescale) alpha = exp2_fast(m_run - next);
+          m_run = next;
         }
         const float base = m_run == -INFINITY ? 0.0f : m_run;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        // second pass: P, which takes the place of S behind the read
+        const float2 cm2 = make_float2(cm, cm), base2 = make_float2(-base, -base);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t u[64], pk[32];
+          tmem_ld64(lane_base + s_col + 64 * half, u);
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 x = ffma2(make_float2(sv[32 * cc + 2 * e], sv[32 * cc + 2 * e + 1]), make_float2(cm, cm),
-                                   make_float2(-base, -base));
-            const float p0 = exp2_fast(x.x), p1 = exp2_fast(x.y);
-            sum[cc] += p0 + p1;
-            pk[e] = Elem16<T>::pack(p0, p1);
+          for (int e = 0; e < 32; ++e) {
+            float2 x = ffma2(make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1])), cm2, base2);
+            if (xt_poly_pair(e % 16)) {
+              x = exp2_poly<F16 ? 4 : 3>(x);
+            } else {
+              x.x = exp2_fast(x.x);
+              x.y = exp2_fast(x.y);
+            }
+            sum[e & 1] = fadd2(sum[e & 1], x);
+            pk[e] = Elem16<T>::pack(x.x, x.y);
           }
-          tmem_st16(lane_base + s_col + 16 * cc, pk);
+          tmem_st32(lane_base + s_col + 32 * half, pk);
         }
-        l_run = fmaf(l_run, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+        const float2 all = fadd2(sum[0], sum[1]);
+        l_run = fmaf(l_run, alpha, all.x + all.y);
         // O is stable here: S(j) being complete means PV(j - 1) is
-        if (any && __any_sync(0xffffffffu, rescale)) {
-#pragma unroll
+        if (!first && __any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
           for (int cc = 0; cc < D / 16; ++cc) {
             uint32_t u[16];
             tmem_ld16(lane_base + o_col + 16 * cc, u);
@@ -675,271 +811,292 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
             tmem_st16(lane_base + o_col + 16 * cc, u);
           }
         }
-        any = true;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
-        ++step;
       }
-      if (!ok) break;
+      if (!(st.flags & XS_LAST)) continue;
+      const bool any = !(st.flags & XS_EMPTY);
       if (any) {
-        if (!mbar_wait(&o_full[t], out_no & 1, abort_flag, ERR_WAIT_SOFTMAX)) { ok = false; break; }
+        if (!mbar_wait_s(smem_u32(&o_full[t]), out_no & 1, abort_addr, ERR_WAIT_SOFTMAX)) break;
         ++out_no;
         tc_fence_after();
       }
       // a row that saw no key is zero (its sum is 0, never NaN)
       const bool empty = l_run == 0.0f;
       const float inv = 1.0f / l_run;
-#pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
-        uint32_t o[32];
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-          uint32_t u[16];
-          if (any) {
-            tmem_ld16(lane_base + o_col + 64 * h + 16 * cc, u);
-            tmem_wait_ld_regs(u);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            o[8 * cc + e] = empty ? 0u : Elem16<T>::pack(__uint_as_float(u[2 * e]) * inv, __uint_as_float(u[2 * e + 1]) * inv);
+      T* dst = static_cast<T*>(p.out) + (((long long)st.b * p.lq + tok) * p.heads + head) * D;
+#pragma unroll 2
+      for (int cc = 0; cc < D / 16; ++cc) {
+        uint32_t u[16], o[8];
+        if (any) {
+          tmem_ld16(lane_base + o_col + 16 * cc, u);
+          tmem_wait_ld_regs(u);
         }
-        if (stored && r == 0) bulk_wait_read();
-        named_sync(1 + t);
-        // the 128-byte swizzle of the store's tensor map
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          *reinterpret_cast<uint4*>(stage + r * 128 + ((x ^ (r & 7)) << 4)) =
-              make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-        fence_proxy_async_smem();
-        named_sync(1 + t);
-        if (r == 0 && it.q0 + t * qstep < p.lq) {
-          tma_store_4d(&maps.o, stage, 64 * h, it.q0 + t * qstep, head, it.b);
-          bulk_commit();
-        }
-        stored = true;
+        for (int e = 0; e < 8; ++e)
+          o[e] = empty ? 0u : Elem16<T>::pack(__uint_as_float(u[2 * e]) * inv, __uint_as_float(u[2 * e + 1]) * inv);
+        if (tok < p.lq) st_global_32b(dst + 16 * cc, o);
       }
     }
-    if (r == 0) bulk_wait_all();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 0) {
       // ----------------------------------------------------------- loads
-      if (lane == 0) {
-        bool ok = true;
-        int load = 0, nq = 0;
-        for (int i = begin; i < end && ok; ++i) {
-          const CrossItem it = cross_item(P, i, begin, end, NS);
-          const bool fetch = !it.resident || it.run_first;
-          int j = cross_next_tile(P, it, 0);
-          if (j < it.tiles) {
+      CrossStep st;
+      bool ok = true;
+      for (uint32_t no = 0; ok && read_step(no, st, rec_ready(no)); ++no) {
+        if (lane == 0 && !(st.flags & XS_EMPTY)) {
+          if (st.flags & XS_FIRST) {
 #pragma unroll 1
             for (int t = 0; t < 2 && ok; ++t) {
-              if (nq > 0 && !mbar_wait(&q_empty[t], (nq - 1) & 1, abort_flag, ERR_WAIT_LOAD)) { ok = false; break; }
+              if (st.item_no > 0 && !mbar_wait_fast(smem_u32(&q_empty[t]), (st.item_no - 1) & 1, abort_addr, ERR_WAIT_LOAD)) {
+                ok = false;
+                break;
+              }
               mbar_arrive_expect_tx(&q_full[t], X::TILE);
               for (int h = 0; h < HALVES; ++h)
-                tma_load_4d(smem + X::OFF_Q + t * X::TILE + h * BOX, &maps.q, &q_full[t], 64 * h, it.q0 + t * qstep,
-                            it.h0 + t * hstep, it.b);
-              q_loaded[t] = nq + 1;
+                tma_load_4d(smem + X::OFF_Q + t * X::TILE + h * BOX, &maps.q, &q_full[t], 64 * h, st.q0 + t * qstep,
+                            st.h0 + t * hstep, st.b);
+              q_loads[t] = st.item_no + 1;
             }
-            ++nq;
-            for (; j < it.tiles && fetch && ok; j = cross_next_tile(P, it, j + 1)) {
-              const int s = load % NS;
-              const uint32_t ph = (load / NS) & 1;
-              if (load >= NS && !mbar_wait(&k_empty[s], ph ^ 1, abort_flag, ERR_WAIT_LOAD)) { ok = false; break; }
+          }
+          if (ok && (st.flags & XS_LOAD)) {
+            const int s = st.load % NS, kb = p.k_sb == 0 ? 0 : st.b;
+            const uint32_t ph = (st.load / NS) & 1;
+            ok = st.load < NS || mbar_wait_fast(smem_u32(&k_empty[s]), ph ^ 1, abort_addr, ERR_WAIT_LOAD);
+            if (ok) {
               mbar_arrive_expect_tx(&k_full[s], X::TILE);
               for (int h = 0; h < HALVES; ++h)
-                tma_load_4d(smem + X::OFF_K + s * X::TILE + h * BOX, &maps.k, &k_full[s], 64 * h, j * XT_BN, it.hk,
-                            shared_kv ? 0 : it.b);
-              loaded = 2 * load + 1;
-              if (load >= NS && !mbar_wait(&v_empty[s], ph ^ 1, abort_flag, ERR_WAIT_LOAD)) { ok = false; break; }
+                tma_load_4d(smem + X::OFF_K + s * X::TILE + h * BOX, &maps.k, &k_full[s], 64 * h, st.j * XT_BN, st.hk, kb);
+              k_loads = st.load + 1;
+              ok = st.load < NS || mbar_wait_fast(smem_u32(&v_empty[s]), ph ^ 1, abort_addr, ERR_WAIT_LOAD);
+            }
+            if (ok) {
               mbar_arrive_expect_tx(&v_full[s], X::TILE);
               for (int h = 0; h < HALVES; ++h)
-                tma_load_4d(smem + X::OFF_V + s * X::TILE + h * BOX, &maps.v, &v_full[s], 64 * h, j * XT_BN, it.hk,
-                            shared_kv ? 0 : it.b);
-              loaded = 2 * load + 2;
-              ++load;
+                tma_load_4d(smem + X::OFF_V + s * X::TILE + h * BOX, &maps.v, &v_full[s], 64 * h, st.j * XT_BN, st.hk, kb);
+              v_loads = st.load + 1;
             }
           }
         }
+        ok = __all_sync(0xffffffffu, ok);
       }
     } else if (warp == 1) {
       // -------------------------------------------------------- products
-      if (lane == 0) {
-        constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0 : 1;
-        constexpr uint32_t idesc_s = make_idesc(1, fmt, fmt, 0, 0, XT_BM, XT_BN);  // Q K^T, both K-major
-        constexpr uint32_t idesc_o = make_idesc(1, fmt, fmt, 0, 1, XT_BM, D);      // P V, V MN-major
-        // One step: tile j of item i, its ring slot `load`.
-        struct Step {
-          int i, j, load, item_no;
-          bool first, last, release;
-        };
-        CrossItem it;
-        int run_base = 0, next_load = 0, item_no = -1;
-        auto open_item = [&](Step& st) {  // first step at or after item st.i
-          for (; st.i < end; ++st.i) {
-            it = cross_item(P, st.i, begin, end, NS);
-            const int j = cross_next_tile(P, it, 0);
-            if (it.resident && it.run_first) run_base = next_load, next_load += it.tiles;
-            if (j >= it.tiles) continue;
-            ++item_no;
-            st.j = j;
-            st.first = true;
-            st.item_no = item_no;
-            return true;
-          }
-          return false;
-        };
-        auto close_step = [&](Step& st) {  // ring slot, whether it is the item's last, whether it frees the slot
-          st.load = it.resident ? run_base + st.j : next_load++;
-          st.last = cross_next_tile(P, it, st.j + 1) >= it.tiles;
-          st.release = !it.resident || it.run_last;
-        };
-        auto advance = [&](Step& st) {
-          if (!st.last) {
-            st.j = cross_next_tile(P, it, st.j + 1);
-            st.first = false;
-          } else {
-            ++st.i;
-            if (!open_item(st)) return false;
-          }
-          close_step(st);
-          return true;
-        };
-        auto issue_s = [&](int t, const Step& st) {
-          const int s = st.load % NS;
-          // 16 columns further: 32 B on within a 64-column half, BOX on to the next (descriptors count 16 B)
-          const uint64_t qa = umma_desc_sw128(smem_u32(smem + X::OFF_Q + t * X::TILE), 16, 1024);
-          const uint64_t ka = umma_desc_sw128(smem_u32(smem + X::OFF_K + s * X::TILE), 16, 1024);
+      constexpr uint32_t fmt = F16 ? 0 : 1;
+      constexpr uint32_t idesc_s = make_idesc(1, fmt, fmt, 0, 0, XT_BM, XT_BN);  // Q K^T, both K-major
+      constexpr uint32_t idesc_o = make_idesc(1, fmt, fmt, 0, 1, XT_BM, D);      // P V, V MN-major
+      const uint32_t base = warp_uniform(smem_u32(smem));
+      const uint32_t tm = warp_uniform(tmem);
+      auto wait = [&](const uint64_t* bar, uint32_t parity) {
+        return mbar_wait_fast(smem_u32(bar), parity, abort_addr, ERR_WAIT_MMA);
+      };
+      auto all = [](bool v) { return __all_sync(0xffffffffu, v) != 0; };
+      // S_t of the step with ring slot s: 16 columns further are 32 B on within
+      // a 64-column half, BOX on to the next (descriptors count 16 B)
+      auto issue_s = [&](int t, int s, int flags) {
+        const uint64_t qa = umma_desc_sw128(base + X::OFF_Q + t * X::TILE, 16, 1024);
+        const uint64_t ka = umma_desc_sw128(base + X::OFF_K + s * X::TILE, 16, 1024);
+        if (leader) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
-            mma_bf16_ss(tmem + t * 128, qa + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
+            mma_bf16_ss(tm + t * 128, qa + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
           }
           mma_commit(&s_full[t]);
-          if (st.last) mma_commit(&q_empty[t]);
-          if (t == 1 && st.release) mma_commit(&k_empty[s]);
-        };
-        Step cur;
-        cur.i = begin;
-        bool have = open_item(cur);
-        if (have) close_step(cur);
-        bool ok = have;
-        if (ok) ok = mbar_wait(&k_full[cur.load % NS], (cur.load / NS) & 1, abort_flag, ERR_WAIT_MMA);
-#pragma unroll 1
-        for (int t = 0; t < 2 && ok; ++t) {
-          ok = mbar_wait(&q_full[t], 0, abort_flag, ERR_WAIT_MMA);
+          if (flags & XS_LAST) mma_commit(&q_empty[t]);
+          if (t == 1 && (flags & XS_FREE)) mma_commit(&k_empty[s]);
+        }
+        __syncwarp();
+      };
+      uint32_t no = 0;
+      // the next step that has products
+      auto next = [&](CrossStep& st) {
+        do {
+          if (!read_step(no, st, rec_ready(no))) return false;
+          ++no;
+        } while (st.flags & XS_EMPTY);
+        st.flags = warp_uniform(st.flags);
+        st.load = warp_uniform(st.load);
+        st.item_no = warp_uniform(st.item_no);
+        return true;
+      };
+      CrossStep cur, nxt;
+      bool have = next(cur);
+      bool ok = have && all(wait(&k_full[cur.load % NS], (cur.load / NS) & 1));
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        ok = ok && all(wait(&q_full[t], 0));
+        tc_fence_after();
+        if (ok) issue_s(t, cur.load % NS, cur.flags);
+      }
+      for (uint32_t step = 0; have && ok; ++step) {
+        const bool more = next(nxt);
+        const int s = cur.load % NS;
+        const uint32_t ph = (cur.load / NS) & 1;
+        ok = wait(&v_full[s], ph) && wait(&aux_full[s], ph);
+        if (more) ok = ok && wait(&k_full[nxt.load % NS], (nxt.load / NS) & 1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          ok = all(ok && wait(&p_full[t], step & 1));
           if (!ok) break;
           tc_fence_after();
-          issue_s(t, cur);
-        }
-        for (uint32_t step = 0; have && ok; ++step) {
-          Step nxt = cur;
-          const bool more = advance(nxt);
-          const int s = cur.load % NS;
-          const uint32_t ph = (cur.load / NS) & 1;
-#pragma unroll 1
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (t == 0 && !(mbar_wait(&v_full[s], ph, abort_flag, ERR_WAIT_MMA) &&
-                            mbar_wait(&aux_full[s], ph, abort_flag, ERR_WAIT_MMA))) { ok = false; break; }
-            if (!mbar_wait(&p_full[t], step & 1, abort_flag, ERR_WAIT_MMA)) { ok = false; break; }
-            tc_fence_after();
-            // 16 keys further: 16 rows of 128 B; the two 64-column halves are BOX apart (LBO)
-            const uint64_t va = umma_desc_sw128(smem_u32(smem + X::OFF_V + s * X::TILE), BOX, 1024);
+          // 16 keys further: 16 rows of 128 B; the two 64-column halves are BOX apart (LBO)
+          const uint64_t va = umma_desc_sw128(base + X::OFF_V + s * X::TILE, BOX, 1024);
+          if (leader) {
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
-              mma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, va + kk * (2048 >> 4), idesc_o,
-                          (!cur.first || kk > 0) ? 1u : 0u);
-            if (cur.last) mma_commit(&o_full[t]);
-            if (t == 1 && cur.release) mma_commit(&v_empty[s]);
-            if (more) {
-              if (t == 0 && !mbar_wait(&k_full[nxt.load % NS], (nxt.load / NS) & 1, abort_flag, ERR_WAIT_MMA)) { ok = false; break; }
-              if (nxt.first && !mbar_wait(&q_full[t], nxt.item_no & 1, abort_flag, ERR_WAIT_MMA)) { ok = false; break; }
-              tc_fence_after();
-              issue_s(t, nxt);
-            }
+              mma_bf16_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, va + kk * (2048 >> 4), idesc_o,
+                          kk > 0 || !(cur.flags & XS_FIRST) ? 1u : 0u);
+            if (cur.flags & XS_LAST) mma_commit(&o_full[t]);
+            if (t == 1 && (cur.flags & XS_FREE)) mma_commit(&v_empty[s]);
           }
-          cur = nxt;
-          have = more;
+          __syncwarp();
+          if (more) {
+            if (nxt.flags & XS_FIRST) ok = all(wait(&q_full[t], nxt.item_no & 1));
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(t, nxt.load % NS, nxt.flags);
+          }
         }
+        cur = nxt;
+        have = more;
       }
     } else if (warp == 2) {
       // ---------------------------------------- side data of every K/V load
-      bool ok = true;
-      int load = 0;
-      for (int i = begin; i < end && ok; ++i) {
-        const CrossItem it = cross_item(P, i, begin, end, NS);
-        if (it.resident && !it.run_first) continue;
+      CrossStep st;
+      for (uint32_t no = 0; read_step(no, st, rec_ready(no)); ++no) {
+        if (!(st.flags & XS_LOAD)) continue;
+        const int s = st.load % NS, n = cross_keys(p, st.b);
         const bool key_mask = p.mask && !P.bits;
-        for (int j = cross_next_tile(P, it, 0); j < it.tiles; j = cross_next_tile(P, it, j + 1)) {
-          const int s = load % NS;
-          float add[4];
-          uint32_t word[4];
-          bool plain = true;
+        float add[4];
+        uint32_t word[4];
+        bool plain = true;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int key = j * XT_BN + 32 * c + lane;
-            bool keep = key < it.n;
-            add[c] = 0.0f;
-            if (keep && p.bias) {
-              const float raw = __ldg(p.bias + it.b * p.bias_sb + key);
-              keep = raw != -INFINITY;
-              // log2 units; a finite addend stays finite
-              add[c] = raw * kLog2e;
-              if (fabsf(raw) <= 3.4028234663852886e38f) add[c] = fminf(fmaxf(add[c], -3.4028234663852886e38f), 3.4028234663852886e38f);
-              if (!keep) add[c] = 0.0f;
+        for (int c = 0; c < 4; ++c) {
+          const int key = st.j * XT_BN + 32 * c + lane;
+          bool keep = key < n;
+          add[c] = 0.0f;
+          if (keep && p.bias) {
+            const float raw = __ldg(p.bias + st.b * p.bias_sb + key);
+            keep = raw != -INFINITY;
+            // log2 units; a finite addend stays finite
+            add[c] = raw * kLog2e;
+            if (fabsf(raw) <= 3.4028234663852886e38f) add[c] = fminf(fmaxf(add[c], -3.4028234663852886e38f), 3.4028234663852886e38f);
+            if (!keep) add[c] = 0.0f;
+          }
+          if (keep && key_mask) keep = __ldg(p.mask + st.b * p.m_sb + key * p.m_sk) != 0;
+          word[c] = __ballot_sync(0xffffffffu, keep);
+          plain = plain && !__any_sync(0xffffffffu, add[c] != 0.0f);
+        }
+        uint4 live = make_uint4(word[0], word[1], word[2], word[3]);
+        if (P.bits) {
+          const uint4 seen = cross_seen(P, st.b, st.h0, st.q0, st.j);
+          live.x &= seen.x, live.y &= seen.y, live.z &= seen.z, live.w &= seen.w;
+        }
+        // the previous user of the slot is done once V has been loaded over it
+        if (!__all_sync(0xffffffffu, mbar_wait_fast(smem_u32(&v_full[s]), (st.load / NS) & 1, abort_addr, ERR_WAIT_LOAD))) break;
+        uint8_t* aux = smem + X::OFF_AUX + s * X::AUX;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) reinterpret_cast<float*>(aux)[32 * c + lane] = add[c];
+        if (lane == 0) {
+          *reinterpret_cast<uint4*>(aux + 512) = make_uint4(word[0], word[1], word[2], word[3]);
+          *reinterpret_cast<int*>(aux + 528) = plain ? 0 : 1;
+        }
+        // V rows of keys that nobody sees
+        const uint32_t lw[4] = {live.x, live.y, live.z, live.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (!((lw[c] >> lane) & 1u)) {
+            uint8_t* row = smem + X::OFF_V + s * X::TILE + (32 * c + lane) * 128;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+              for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(row + h * BOX + 16 * x) = make_uint4(0, 0, 0, 0);
+          }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&aux_full[s]);
+      }
+    } else if (lane == 0) {
+      // -------------------------------------------------------- the walk
+      int range[2];
+      cross_range(P, range);
+      const int per = P.pairs * P.qtiles;
+      int load = 0, item_no = 0, run_base = 0;
+      uint32_t no = 0;
+      auto put = [&](const CrossStep& st) {
+        const uint32_t at = no % XT_RECORDS;
+        if (no >= XT_RECORDS && !mbar_wait_fast(smem_u32(&rec_empty[at]), ((no / XT_RECORDS) & 1) ^ 1, abort_addr, ERR_WAIT_LOAD)) return false;
+        records[2 * at] = make_int4(st.flags, st.j, st.load, st.item_no);
+        records[2 * at + 1] = make_int4(st.b, st.hk, st.h0, st.q0);
+        mbar_arrive(&rec_full[at]);
+        ++no;
+        return true;
+      };
+      bool ok = true;
+      CrossStep st;
+      for (int i = range[0]; i < range[1] && ok; ++i) {
+        const int key = i / per, rem = i % per;
+        const int pair = rem / P.qtiles, qt = rem % P.qtiles;
+        st.b = key / p.kvheads;
+        st.hk = key % p.kvheads;
+        st.h0 = st.hk * p.group + (P.qpair ? pair : 2 * pair);
+        st.q0 = qt * (P.qpair ? 2 * XT_BM : XT_BM);
+        const int tiles = (cross_keys(p, st.b) + XT_BN - 1) / XT_BN;
+        const bool run_first = i == range[0] || rem == 0, run_last = i == range[1] - 1 || rem == per - 1;
+        // K and V of a run of items stay when all their tiles fit the ring
+        // (not under a packed mask: which V rows are zeroed depends on the item)
+        const bool resident = !P.bits && tiles <= NS;
+        if (resident && run_first) run_base = load, load += tiles;
+        auto next_tile = [&](int j) {
+          if (P.bits)
+            for (; j < tiles; ++j) {
+              const uint4 w = cross_seen(P, st.b, st.h0, st.q0, j);
+              if (w.x | w.y | w.z | w.w) break;
             }
-            if (keep && key_mask) keep = __ldg(p.mask + it.b * p.m_sb + key * p.m_sk) != 0;
-            word[c] = __ballot_sync(0xffffffffu, keep);
-            plain = plain && !__any_sync(0xffffffffu, add[c] != 0.0f);
-          }
-          uint4 live = make_uint4(word[0], word[1], word[2], word[3]);
-          if (P.bits) {
-            const uint4 seen = cross_seen(P, it, j);
-            live.x &= seen.x, live.y &= seen.y, live.z &= seen.z, live.w &= seen.w;
-          }
-          if (!mbar_wait(&v_full[s], (load / NS) & 1, abort_flag, ERR_WAIT_LOAD)) { ok = false; break; }
-          uint8_t* aux = smem + X::OFF_AUX + s * X::AUX;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) reinterpret_cast<float*>(aux)[32 * c + lane] = add[c];
-          if (lane == 0) {
-            *reinterpret_cast<uint4*>(aux + 512) = make_uint4(word[0], word[1], word[2], word[3]);
-            *reinterpret_cast<int*>(aux + 528) = plain ? 0 : 1;
-          }
-          // V rows of keys that nobody sees
-          const uint32_t lw[4] = {live.x, live.y, live.z, live.w};
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (!((lw[c] >> lane) & 1u)) {
-              uint8_t* row = smem + X::OFF_V + s * X::TILE + (32 * c + lane) * 128;
-#pragma unroll
-              for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-                for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(row + h * BOX + 16 * x) = make_uint4(0, 0, 0, 0);
-            }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&aux_full[s]);
-          ++load;
+          return j;
+        };
+        st.j = next_tile(0);
+        st.item_no = item_no;
+        if (st.j >= tiles) {
+          st.flags = XS_FIRST | XS_LAST | XS_EMPTY;
+          st.load = 0;
+          ok = put(st);
+          continue;
+        }
+        ++item_no;
+        for (int j = st.j, first = 1; j < tiles && ok; first = 0) {
+          const int after = next_tile(j + 1);
+          st.j = j;
+          st.load = resident ? run_base + j : load++;
+          st.flags = (first ? XS_FIRST : 0) | (after >= tiles ? XS_LAST : 0) | (!resident || run_first ? XS_LOAD : 0) |
+                     (!resident || run_last ? XS_FREE : 0);
+          ok = put(st);
+          j = after;
         }
       }
+      st.flags = XS_END;
+      if (ok) put(st);
     }
   }
 
   // ------------------------------------------------------------ teardown
+  __syncwarp();
   if (*abort_flag) {
     if (warp == 0 && lane == 0) {
       for (int t = 0; t < 2; ++t)
-        if (q_loaded[t]) mbar_drain(&q_full[t], (q_loaded[t] - 1) & 1);
-      const int kl = (loaded + 1) / 2, vl = loaded / 2;
-      for (int x = max(0, kl - NS); x < kl; ++x) mbar_drain(&k_full[x % NS], (x / NS) & 1);
-      for (int x = max(0, vl - NS); x < vl; ++x) mbar_drain(&v_full[x % NS], (x / NS) & 1);
+        if (q_loads[t]) mbar_drain(&q_full[t], (q_loads[t] - 1) & 1);
+      for (int x = max(0, k_loads - NS); x < k_loads; ++x) mbar_drain(&k_full[x % NS], (x / NS) & 1);
+      for (int x = max(0, v_loads - NS); x < v_loads; ++x) mbar_drain(&v_full[x % NS], (x / NS) & 1);
     }
-    if (warp == 1 && lane == 0) {  // behind every product issued
+    if (warp == 1 && leader) {  // behind every product issued
       mma_commit(drained);
       mbar_drain(drained, 0);
     }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();

@@ -139,6 +139,15 @@ __device__ __forceinline__ bool mbar_wait_s(uint32_t a, uint32_t parity, uint32_
     }
   }
 }
+// mbar_wait_s with the waiting loop out of line: a kernel with many waits
+// keeps its instruction footprint, and a wait that need not wait costs one
+// try_wait.
+__device__ __noinline__ bool mbar_wait_slow(uint32_t a, uint32_t parity, uint32_t abort_addr, int code) {
+  return mbar_wait_s(a, parity, abort_addr, code);
+}
+__device__ __forceinline__ bool mbar_wait_fast(uint32_t a, uint32_t parity, uint32_t abort_addr, int code) {
+  return mbar_try_wait(a, parity) || mbar_wait_slow(a, parity, abort_addr, code);
+}
 __device__ __forceinline__ void mbar_arrive_s(uint32_t a) {
   asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(a) : "memory");
 }

@@ -555,7 +555,6 @@ static int cross_tile_launch(const CrossParams& p, void* work, int dim, int dtyp
   int rc = make_map_4d_bf16(&maps.q, p.q, D, p.lq, H, B, p.q_st, p.q_sh, p.q_sb, 64, XT_BM, dt);
   if (!rc) rc = make_map_4d_bf16(&maps.k, p.k, D, p.lk, Hk, shared ? 1 : B, p.k_st, p.k_sh, shared ? D : p.k_sb, 64, XT_BN, dt);
   if (!rc) rc = make_map_4d_bf16(&maps.v, p.v, D, p.lk, Hk, shared ? 1 : B, p.v_st, p.v_sh, shared ? D : p.v_sb, 64, XT_BN, dt);
-  if (!rc) rc = make_map_4d_bf16(&maps.o, p.out, D, p.lq, H, B, H * D, D, (uint64_t)p.lq * H * D, 64, XT_BM, dt);
   if (rc) return rc;
   CrossTileParams P;
   memset(&P, 0, sizeof(P));
@@ -984,7 +983,7 @@ K2B_EXPORT int k2b_cross_attention(const void* q, const void* k, const void* v, 
   if (batch <= 0 || heads <= 0 || kvheads <= 0 || heads % kvheads || lq <= 0 || lk < 0 || (dim != 64 && dim != 128) ||
       (dtype != COND_FP16 && dtype != COND_BF16))
     return (int)cudaErrorInvalidValue;
-  if (!q || !out || !aligned16(q) || !aligned16(out) ||
+  if (!q || !out || !aligned16(q) || reinterpret_cast<uintptr_t>(out) % 32 ||
       (lk > 0 && (!k || !v || !aligned16(k) || !aligned16(v))) ||
       (lengths && reinterpret_cast<uintptr_t>(lengths) % 4) || (bias && reinterpret_cast<uintptr_t>(bias) % 4))
     return (int)cudaErrorInvalidValue;

@@ -225,8 +225,8 @@ int k2b_qk_norm_rope(const void* q, const void* k, const void* wq, const void* w
                      void* qo, void* ko, int batch, int lq, int lk, int heads, int kvheads, int dim, long long q_sb,
                      long long q_sh, long long q_st, long long k_sb, long long k_sh, long long k_st, int fq_batch,
                      int fk_batch, float eps_q, float eps_k, int dtype, void* stream);
-/* out [batch, lq, heads*dim] = softmax(q k^T scale + bias) v over the keys that
- * are not excluded, 0 for a row without any.  Strides as above; k_sb = v_sb = 0
+/* out [batch, lq, heads*dim] (32-byte aligned) = softmax(q k^T scale + bias) v
+ * over the keys that are not excluded, 0 for a row without any.  Strides as above; k_sb = v_sb = 0
  * shares K and V among the batch.  Excluded: keys >= lengths[b] (int32 [batch]
  * or null, clamped to 0..lk), keys with bias -inf (fp32 [batch or 1, lk], batch
  * stride bias_sb, or null), keys whose mask byte is 0 (by byte strides m_sb,
