@@ -323,15 +323,18 @@ __global__ void __launch_bounds__(XF_THREADS) cross_few_kernel(const __grid_cons
 // execute in order, so S of the next tile may overwrite P behind the PV
 // product that reads it, and S(j) being complete implies PV(j - 1) is.
 //
-// Warps: 0 TMA loads, 1 products, 2 per-tile side data, 3 the walk, 4-7 and
-// 8-11 softmax and output of slot 0 and 1 (a thread owns a row).
-//   - Warp 3 alone decides what is next: it writes one record per step (item,
+// Warps: 0 the walk and its TMA loads, 1 and 3 products of slot 0 and 1, 2
+// per-tile side data, 4-7 and 8-11 softmax and output of slot 0 and 1 (a
+// thread owns a row).
+//   - Warp 0 alone decides what is next: it writes one record per step (item,
 //     key tile, ring slot, what to load and free) into a ring that the other
 //     roles read, so that no division, length or mask lookup stands between a
 //     barrier and the product behind it.
-//   - Warp 1 runs as a whole warp with one elected lane issuing: descriptors
-//     are then in uniform registers.  Issued from a one-lane branch, each
-//     product cost 80-100 cycles of scalar work against 64 of tensor time.
+//   - A slot's products are issued by a warp of its own, as a whole warp with
+//     one elected lane: descriptors are then in uniform registers (issued from
+//     a one-lane branch, each product cost 80-100 cycles of scalar work against
+//     64 of tensor time).  PV of a tile and S of the next go out together once
+//     P is there; everything else they need was waited for before.
 //   - Loads run ahead across items.  While a run of items has the same (b, KV
 //     head) and all its tiles fit the ring, K and V stay where they are: a
 //     short prompt is read once per CTA, not once per query tile.
@@ -345,20 +348,13 @@ __global__ void __launch_bounds__(XF_THREADS) cross_few_kernel(const __grid_cons
 //     skipped by every role.
 //   - O is rescaled in TMEM only when a row's maximum grew by more than 2^8
 //     (P and the sum then stay within fp16 and fp32; o = O / l is the same).
-//   - Part of the exponentials run on the FMA pipe (exp2_poly): at 128 x 128
-//     scores per 1024 cycles of tensor time the MUFU alone would take as long
-//     as the products do.
 constexpr int XT_BM = 128;
 constexpr int XT_BN = 128;
 constexpr int XT_THREADS = 384;
-constexpr int XT_LAUNCH_REGS = 168;  // 65536 / 384; split 80 / 208 by setmaxnreg (128 x 80 + 256 x 208 of 384 x 168)
+constexpr int XT_LAUNCH_REGS = 168;  // 65536 / 384; split 88 / 208 by setmaxnreg (128 x 88 + 256 x 208 = 384 x 168)
 constexpr float XT_RESCALE = 8.0f;   // log2 units
 constexpr int XT_RECORDS = 8;        // steps the walk may be ahead of the slowest role
-constexpr int XT_READERS = 11;       // loads, products, side data, eight softmax warps
-constexpr int XT_POLY_PAIRS = 6;     // of the 16 pairs of a 32-key chunk, those that exp2_poly takes
-__host__ __device__ constexpr bool xt_poly_pair(int e) {  // spread evenly over the chunk
-  return (e + 1) * XT_POLY_PAIRS / 16 != e * XT_POLY_PAIRS / 16;
-}
+constexpr int XT_READERS = 11;       // products (2), side data, eight softmax warps
 
 template <int D>
 struct XtShape {
@@ -371,7 +367,7 @@ struct XtShape {
   static constexpr int AUX = 128 * 4 + 32;             // addends, keep words, flags
   static constexpr int OFF_REC = OFF_AUX + STAGES * AUX;
   static constexpr int OFF_BAR = OFF_REC + XT_RECORDS * 32;
-  static constexpr int NBARS = 4 + 5 * STAGES + 7 + 2 * XT_RECORDS;
+  static constexpr int NBARS = 4 + 5 * STAGES + 8 + 2 * XT_RECORDS;
   static constexpr int SMEM = OFF_BAR + NBARS * 8 + 32 + 1024;
 };
 
@@ -435,8 +431,11 @@ enum CrossFlags : int {
   XS_END = 32,
 };
 struct CrossStep {
-  int flags, j, load, item_no;  // load: running number of the K/V load (ring slot load % STAGES)
-  int b, hk, h0, q0;            // slot t: head h0 + t * hstep, tokens q0 + t * qstep..
+  // flags above, and for the products: ring slot << 8, its phase << 12, the
+  // phase of the item's queries << 13
+  int flags;
+  int j, load, item_no;  // load: running number of the K/V load (ring slot load % STAGES)
+  int b, hk, h0, q0;     // slot t: head h0 + t * hstep, tokens q0 + t * qstep..
 };
 
 // The keys of tile j that some row of the item sees (packed mask only).
@@ -520,8 +519,40 @@ __device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
   return r;
 }
 
+// 128 columns of this lane's row, complete on return.
+__device__ __forceinline__ void tmem_ld_row(uint32_t taddr, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, "
+      "%34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, "
+      "%54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, %72, %73, "
+      "%74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, "
+      "%94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
+      "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      :
+        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]),
+        "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]),
+        "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]),
+        "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]),
+        "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]),
+        "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]),
+        "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]),
+        "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]),
+        "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr)
+      : "memory");
+}
 // 64 columns of this lane's row, complete on return.
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+__device__ __forceinline__ void tmem_ld_row(uint32_t taddr, uint32_t (&r)[64]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
       "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, "
@@ -540,27 +571,24 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st64(uint32_t taddr, const uint32_t (&r)[64]) {
+// 32 columns of this lane's row, complete on return.
+__device__ __forceinline__ void tmem_ld_row(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13"
-      ", %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33"
-      ", %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53"
-      ", %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64};"
-      ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(r[32]), "r"(r[33]), "r"(r[34]), "r"(r[35]),
-        "r"(r[36]), "r"(r[37]), "r"(r[38]), "r"(r[39]), "r"(r[40]), "r"(r[41]), "r"(r[42]), "r"(r[43]), "r"(r[44]),
-        "r"(r[45]), "r"(r[46]), "r"(r[47]), "r"(r[48]), "r"(r[49]), "r"(r[50]), "r"(r[51]), "r"(r[52]), "r"(r[53]),
-        "r"(r[54]), "r"(r[55]), "r"(r[56]), "r"(r[57]), "r"(r[58]), "r"(r[59]), "r"(r[60]), "r"(r[61]), "r"(r[62]),
-        "r"(r[63])
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      :
+        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st_row(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13"
-      ", %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
       ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
@@ -568,35 +596,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-
-// 2^x of a pair on the FMA pipe, x at most about 2^7 and not NaN: x = n + f
-// with n the nearest integer (adding 1.5 * 2^23 rounds to it and leaves it in
-// the low bits), 2^f by a minimax polynomial on [-1/2, 1/2] with constant
-// term 1 (fitted for relative error: 1.0e-4 in degree 3, 2.8e-6 in degree 4),
-// n added to the exponent field.  x is cut at -127, where the result is 0
-// exactly, so an excluded key (-inf) adds nothing.  P is rounded to 2^-9
-// (bf16) or 2^-12 (fp16) afterwards, so degree 3 and 4 lose nothing to it.
-template <int DEGREE>
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  static_assert(DEGREE == 3 || DEGREE == 4, "fitted degrees");
-  constexpr float c1 = DEGREE == 3 ? 0.6932829022407532f : 0.6931241750717163f;
-  constexpr float c2 = DEGREE == 3 ? 0.24221095442771912f : 0.24024099111557007f;
-  constexpr float c3 = DEGREE == 3 ? 0.05500892922282219f : 0.055906426161527634f;
-  constexpr float c4 = 0.009582852944731712f;
-  x.x = fmaxf(x.x, -127.0f);
-  x.y = fmaxf(x.y, -127.0f);
-  const float2 y = fadd2(x, make_float2(kRoundMagic, kRoundMagic));
-  // -n as a product: the packed forms have no negation
-  const float2 f = fadd2(x, ffma2(y, make_float2(-1.0f, -1.0f), make_float2(kRoundMagic, kRoundMagic)));
-  float2 r = make_float2(c3, c3);
-  if (DEGREE == 4) r = ffma2(make_float2(c4, c4), f, r);
-  r = ffma2(r, f, make_float2(c2, c2));
-  r = ffma2(r, f, make_float2(c1, c1));
-  r = ffma2(r, f, make_float2(1.0f, 1.0f));
-  return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(y.x) << 23)),
-                     __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(y.y) << 23)));
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(XT_THREADS, 1)
     cross_tile_kernel(const __grid_constant__ CrossMaps maps, const __grid_constant__ CrossTileParams P) {
@@ -620,7 +619,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
   uint64_t* o_full = p_full + 2;         // [2]
   uint64_t* rec_full = o_full + 2;       // [XT_RECORDS]
   uint64_t* rec_empty = rec_full + XT_RECORDS;
-  uint64_t* drained = rec_empty + XT_RECORDS;  // teardown after an abort
+  uint64_t* drained = rec_empty + XT_RECORDS;  // [2] teardown after an abort
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + X::NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int4* records = reinterpret_cast<int4*>(smem + X::OFF_REC);  // two per step
@@ -639,9 +638,9 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], 2);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], 2);
       mbar_init(&aux_full[i], 1);
     }
     for (int i = 0; i < XT_RECORDS; ++i) {
@@ -649,6 +648,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
       mbar_init(&rec_empty[i], XT_READERS);
     }
     mbar_init(drained, 1);
+    mbar_init(drained + 1, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
     const int w4 = warp & 3;
     const int r = 32 * w4 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * w4) << 16);
-    const uint32_t s_col = t * 128, o_col = 256 + t * 128;
+    const uint32_t s_at = lane_base + t * 128, o_at = lane_base + 256 + t * 128;
     const float c = p.scale * kLog2e;
     uint32_t step = 0, out_no = 0;
     float m_run = -INFINITY, l_run = 0.0f;
@@ -717,54 +717,52 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
             !mbar_wait_s(smem_u32(&s_full[t]), step & 1, abort_addr, ERR_WAIT_SOFTMAX)) break;
         ++step;
         tc_fence_after();
-        // The loops below stay rolled, 64 columns a turn: the whole row in
-        // registers makes 90 KB of code, and the kernel then waits for
-        // instructions (hit rate of the SM's instruction cache 74%).
         const uint8_t* aux = smem + X::OFF_AUX + s * X::AUX;
         {
           const uint4 kw = *reinterpret_cast<const uint4*>(aux + 512);
           mine.x &= kw.x, mine.y &= kw.y, mine.z &= kw.z, mine.w &= kw.w;
         }
         const bool adds = *reinterpret_cast<const int*>(aux + 528) != 0;
-        const bool cuts = __any_sync(0xffffffffu, (mine.x & mine.y & mine.z & mine.w) != ~0u);
-        // first pass: the row's maximum; with addends or excluded keys S is
-        // replaced by the scores in log2 units (sv * cm with cm = 1)
-        float mx = -INFINITY;
+        // Scores in log2 units are S * cm.  With addends they replace S first, in
+        // a rolled loop: unrolled it costs the main path its registers, and a
+        // spill here goes to L2 (shared memory leaves L1 next to nothing).
+        float cm = c;
+        if (adds) {
+          cm = 1.0f;
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          uint32_t u[64];
-          tmem_ld64(lane_base + s_col + 64 * half, u);
-          if (adds) {
+          for (int cc = 0; cc < 4; ++cc) {
+            uint32_t u[32];
+            tmem_ld_row(s_at + 32 * cc, u);
 #pragma unroll
-            for (int e = 0; e < 64; e += 4) {
-              const float4 a = *reinterpret_cast<const float4*>(aux + 4 * (64 * half + e));
+            for (int e = 0; e < 32; e += 4) {
+              const float4 a = *reinterpret_cast<const float4*>(aux + 4 * (32 * cc + e));
               u[e] = __float_as_uint(fmaf(__uint_as_float(u[e]), c, a.x));
               u[e + 1] = __float_as_uint(fmaf(__uint_as_float(u[e + 1]), c, a.y));
               u[e + 2] = __float_as_uint(fmaf(__uint_as_float(u[e + 2]), c, a.z));
               u[e + 3] = __float_as_uint(fmaf(__uint_as_float(u[e + 3]), c, a.w));
             }
+            tmem_st_row(s_at + 32 * cc, u);
           }
-          if (cuts) {
-            const uint32_t lo = half ? mine.z : mine.x, hi = half ? mine.w : mine.y;
-#pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if (!(((e < 32 ? lo : hi) >> (e & 31)) & 1u)) u[e] = 0xff800000u;  // -inf
-          }
-          if (adds || cuts) tmem_st64(lane_base + s_col + 64 * half, u);
-          float m4[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            m4[k] = __uint_as_float(u[k]);
-#pragma unroll
-            for (int jj = 1; jj < 15; jj += 2)
-              m4[k] = fmax3_nan(m4[k], __uint_as_float(u[k + 4 * jj]), __uint_as_float(u[k + 4 * jj + 4]));
-            m4[k] = fmax_nan(m4[k], __uint_as_float(u[k + 60]));
-          }
-          mx = fmax3_nan(mx, fmax_nan(m4[0], m4[1]), fmax_nan(m4[2], m4[3]));
+          tmem_wait_st();
         }
-        if (adds || cuts) tmem_wait_st();
-        const float cm = adds ? 1.0f : c;
-        mx *= cm;
+        uint32_t u[128];
+        tmem_ld_row(s_at, u);
+        if (__any_sync(0xffffffffu, (mine.x & mine.y & mine.z & mine.w) != ~0u)) {
+          const uint32_t mw[4] = {mine.x, mine.y, mine.z, mine.w};
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (!((mw[e >> 5] >> (e & 31)) & 1u)) u[e] = 0xff800000u;  // -inf
+        }
+        float m4[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          m4[k] = __uint_as_float(u[k]);
+#pragma unroll
+          for (int jj = 1; jj < 31; jj += 2)
+            m4[k] = fmax3_nan(m4[k], __uint_as_float(u[k + 4 * jj]), __uint_as_float(u[k + 4 * jj + 4]));
+          m4[k] = fmax_nan(m4[k], __uint_as_float(u[k + 124]));
+        }
+        const float mx = cm * fmax_nan(fmax_nan(m4[0], m4[1]), fmax_nan(m4[2], m4[3]));
         // m_run is the reference of P in log2 units: -inf until the row has
         // seen a key, NaN once a score was NaN or +inf (then the row is NaN)
         float alpha = 1.0f;
@@ -776,26 +774,21 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
           m_run = next;
         }
         const float base = m_run == -INFINITY ? 0.0f : m_run;
-        // second pass: P, which takes the place of S behind the read
         const float2 cm2 = make_float2(cm, cm), base2 = make_float2(-base, -base);
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          uint32_t u[64], pk[32];
-          tmem_ld64(lane_base + s_col + 64 * half, u);
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            float2 x = ffma2(make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1])), cm2, base2);
-            if (xt_poly_pair(e % 16)) {
-              x = exp2_poly<F16 ? 4 : 3>(x);
-            } else {
-              x.x = exp2_fast(x.x);
-              x.y = exp2_fast(x.y);
-            }
+            const int at = 64 * cc + 2 * e;
+            float2 x = ffma2(make_float2(__uint_as_float(u[at]), __uint_as_float(u[at + 1])), cm2, base2);
+            x.x = exp2_fast(x.x);
+            x.y = exp2_fast(x.y);
             sum[e & 1] = fadd2(sum[e & 1], x);
             pk[e] = Elem16<T>::pack(x.x, x.y);
           }
-          tmem_st32(lane_base + s_col + 32 * half, pk);
+          tmem_st_row(s_at + 32 * cc, pk);
         }
         const float2 all = fadd2(sum[0], sum[1]);
         l_run = fmaf(l_run, alpha, all.x + all.y);
@@ -804,11 +797,11 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
 #pragma unroll 1
           for (int cc = 0; cc < D / 16; ++cc) {
             uint32_t u[16];
-            tmem_ld16(lane_base + o_col + 16 * cc, u);
+            tmem_ld16(o_at + 16 * cc, u);
             tmem_wait_ld_regs(u);
 #pragma unroll
             for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * alpha);
-            tmem_st16(lane_base + o_col + 16 * cc, u);
+            tmem_st16(o_at + 16 * cc, u);
           }
         }
         tmem_wait_st();
@@ -827,64 +820,122 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
       const bool empty = l_run == 0.0f;
       const float inv = 1.0f / l_run;
       T* dst = static_cast<T*>(p.out) + (((long long)st.b * p.lq + tok) * p.heads + head) * D;
-#pragma unroll 2
-      for (int cc = 0; cc < D / 16; ++cc) {
-        uint32_t u[16], o[8];
-        if (any) {
-          tmem_ld16(lane_base + o_col + 16 * cc, u);
-          tmem_wait_ld_regs(u);
-        }
+#pragma unroll 1
+      for (int cc = 0; cc < D / 64; ++cc) {
+        uint32_t u[64];
+        tmem_ld_row(o_at + 64 * cc, u);  // (of an item without keys: not used)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          o[e] = empty ? 0u : Elem16<T>::pack(__uint_as_float(u[2 * e]) * inv, __uint_as_float(u[2 * e + 1]) * inv);
-        if (tok < p.lq) st_global_32b(dst + 16 * cc, o);
+        for (int x = 0; x < 4; ++x) {
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            o[e] = empty ? 0u : Elem16<T>::pack(__uint_as_float(u[16 * x + 2 * e]) * inv, __uint_as_float(u[16 * x + 2 * e + 1]) * inv);
+          if (tok < p.lq) st_global_32b(dst + 64 * cc + 16 * x, o);
+        }
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 0) {
-      // ----------------------------------------------------------- loads
-      CrossStep st;
-      bool ok = true;
-      for (uint32_t no = 0; ok && read_step(no, st, rec_ready(no)); ++no) {
-        if (lane == 0 && !(st.flags & XS_EMPTY)) {
+      // --------------------------------------------- the walk and its loads
+      if (lane == 0) {
+        int range[2];
+        cross_range(P, range);
+        const int per = P.pairs * P.qtiles;
+        int load = 0, item_no = 0, run_base = 0;
+        uint32_t no = 0;
+        auto put = [&](const CrossStep& st) {
+          const uint32_t at = no % XT_RECORDS;
+          if (no >= XT_RECORDS && !mbar_wait_fast(smem_u32(&rec_empty[at]), ((no / XT_RECORDS) & 1) ^ 1, abort_addr, ERR_WAIT_LOAD)) return false;
+          records[2 * at] = make_int4(st.flags | (st.load % NS) << 8 | ((st.load / NS) & 1) << 12 | (st.item_no & 1) << 13, st.j,
+                                      st.load, st.item_no);
+          records[2 * at + 1] = make_int4(st.b, st.hk, st.h0, st.q0);
+          mbar_arrive(&rec_full[at]);
+          ++no;
+          return true;
+        };
+        // a bounded wait for a place that a load may overwrite
+        auto free_for = [&](const uint64_t* bar, uint32_t parity) {
+          return mbar_wait_fast(smem_u32(bar), parity, abort_addr, ERR_WAIT_LOAD);
+        };
+        // D / 64 boxes of 128 rows from row y of head z
+        auto fetch_tile = [&](const CUtensorMap* map, uint64_t* full, uint8_t* dst, int y, int z, int w) {
+          mbar_arrive_expect_tx(full, X::TILE);
+#pragma unroll 1
+          for (int h = 0; h < HALVES; ++h) tma_load_4d(dst + h * BOX, map, full, 64 * h, y, z, w);
+        };
+        // what step st loads: the item's queries with its first tile, its K and V
+        auto loads_of = [&](const CrossStep& st) {
+          const int s = st.load % NS, kb = p.k_sb == 0 ? 0 : st.b;
+          const uint32_t ph = ((st.load / NS) & 1) ^ 1;
+          if (st.flags & XS_LOAD) {
+            if (st.load >= NS && !free_for(&k_empty[s], ph)) return false;
+            fetch_tile(&maps.k, &k_full[s], smem + X::OFF_K + s * X::TILE, st.j * XT_BN, st.hk, kb);
+            k_loads = st.load + 1;
+          }
           if (st.flags & XS_FIRST) {
 #pragma unroll 1
-            for (int t = 0; t < 2 && ok; ++t) {
-              if (st.item_no > 0 && !mbar_wait_fast(smem_u32(&q_empty[t]), (st.item_no - 1) & 1, abort_addr, ERR_WAIT_LOAD)) {
-                ok = false;
-                break;
-              }
-              mbar_arrive_expect_tx(&q_full[t], X::TILE);
-              for (int h = 0; h < HALVES; ++h)
-                tma_load_4d(smem + X::OFF_Q + t * X::TILE + h * BOX, &maps.q, &q_full[t], 64 * h, st.q0 + t * qstep,
-                            st.h0 + t * hstep, st.b);
+            for (int t = 0; t < 2; ++t) {
+              if (st.item_no > 0 && !free_for(&q_empty[t], (st.item_no - 1) & 1)) return false;
+              fetch_tile(&maps.q, &q_full[t], smem + X::OFF_Q + t * X::TILE, st.q0 + t * qstep, st.h0 + t * hstep, st.b);
               q_loads[t] = st.item_no + 1;
             }
           }
-          if (ok && (st.flags & XS_LOAD)) {
-            const int s = st.load % NS, kb = p.k_sb == 0 ? 0 : st.b;
-            const uint32_t ph = (st.load / NS) & 1;
-            ok = st.load < NS || mbar_wait_fast(smem_u32(&k_empty[s]), ph ^ 1, abort_addr, ERR_WAIT_LOAD);
-            if (ok) {
-              mbar_arrive_expect_tx(&k_full[s], X::TILE);
-              for (int h = 0; h < HALVES; ++h)
-                tma_load_4d(smem + X::OFF_K + s * X::TILE + h * BOX, &maps.k, &k_full[s], 64 * h, st.j * XT_BN, st.hk, kb);
-              k_loads = st.load + 1;
-              ok = st.load < NS || mbar_wait_fast(smem_u32(&v_empty[s]), ph ^ 1, abort_addr, ERR_WAIT_LOAD);
-            }
-            if (ok) {
-              mbar_arrive_expect_tx(&v_full[s], X::TILE);
-              for (int h = 0; h < HALVES; ++h)
-                tma_load_4d(smem + X::OFF_V + s * X::TILE + h * BOX, &maps.v, &v_full[s], 64 * h, st.j * XT_BN, st.hk, kb);
-              v_loads = st.load + 1;
-            }
+          if (st.flags & XS_LOAD) {
+            if (st.load >= NS && !free_for(&v_empty[s], ph)) return false;
+            fetch_tile(&maps.v, &v_full[s], smem + X::OFF_V + s * X::TILE, st.j * XT_BN, st.hk, kb);
+            v_loads = st.load + 1;
+          }
+          return true;
+        };
+        bool ok = true;
+        CrossStep st;
+        for (int i = range[0]; i < range[1] && ok; ++i) {
+          const int key = i / per, rem = i % per;
+          const int pair = rem / P.qtiles, qt = rem % P.qtiles;
+          st.b = key / p.kvheads;
+          st.hk = key % p.kvheads;
+          st.h0 = st.hk * p.group + (P.qpair ? pair : 2 * pair);
+          st.q0 = qt * (P.qpair ? 2 * XT_BM : XT_BM);
+          const int tiles = (cross_keys(p, st.b) + XT_BN - 1) / XT_BN;
+          const bool run_first = i == range[0] || rem == 0, run_last = i == range[1] - 1 || rem == per - 1;
+          // K and V of a run of items stay when all their tiles fit the ring
+          // (not under a packed mask: which V rows are zeroed depends on the item)
+          const bool resident = !P.bits && tiles <= NS;
+          if (resident && run_first) run_base = load, load += tiles;
+          auto next_tile = [&](int j) {
+            if (P.bits)
+              for (; j < tiles; ++j) {
+                const uint4 w = cross_seen(P, st.b, st.h0, st.q0, j);
+                if (w.x | w.y | w.z | w.w) break;
+              }
+            return j;
+          };
+          st.j = next_tile(0);
+          st.item_no = item_no;
+          if (st.j >= tiles) {
+            st.flags = XS_FIRST | XS_LAST | XS_EMPTY;
+            st.load = 0;
+            ok = put(st);
+            continue;
+          }
+          ++item_no;
+          for (int j = st.j, first = 1; j < tiles && ok; first = 0) {
+            const int after = next_tile(j + 1);
+            st.j = j;
+            st.load = resident ? run_base + j : load++;
+            st.flags = (first ? XS_FIRST : 0) | (after >= tiles ? XS_LAST : 0) | (!resident || run_first ? XS_LOAD : 0) |
+                       (!resident || run_last ? XS_FREE : 0);
+            ok = put(st) && loads_of(st);
+            j = after;
           }
         }
-        ok = __all_sync(0xffffffffu, ok);
+        st.flags = XS_END;
+        if (ok) put(st);
       }
-    } else if (warp == 1) {
-      // -------------------------------------------------------- products
+    } else if (warp != 2) {
+      // ------------------------------------------- products of slot t
+      const int t = warp >> 1;
       constexpr uint32_t fmt = F16 ? 0 : 1;
       constexpr uint32_t idesc_s = make_idesc(1, fmt, fmt, 0, 0, XT_BM, XT_BN);  // Q K^T, both K-major
       constexpr uint32_t idesc_o = make_idesc(1, fmt, fmt, 0, 1, XT_BM, D);      // P V, V MN-major
@@ -893,78 +944,80 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
       auto wait = [&](const uint64_t* bar, uint32_t parity) {
         return mbar_wait_fast(smem_u32(bar), parity, abort_addr, ERR_WAIT_MMA);
       };
-      auto all = [](bool v) { return __all_sync(0xffffffffu, v) != 0; };
-      // S_t of the step with ring slot s: 16 columns further are 32 B on within
-      // a 64-column half, BOX on to the next (descriptors count 16 B)
-      auto issue_s = [&](int t, int s, int flags) {
-        const uint64_t qa = umma_desc_sw128(base + X::OFF_Q + t * X::TILE, 16, 1024);
-        const uint64_t ka = umma_desc_sw128(base + X::OFF_K + s * X::TILE, 16, 1024);
-        if (leader) {
+      const uint64_t q_desc = umma_desc_sw128(base + X::OFF_Q + t * X::TILE, 16, 1024);
+      const uint64_t k_desc = umma_desc_sw128(base + X::OFF_K, 16, 1024);
+      const uint64_t v_desc = umma_desc_sw128(base + X::OFF_V, BOX, 1024);
+      // PV of step w: 16 keys further are 16 rows of 128 B, the two 64-column
+      // halves BOX apart (LBO); descriptors count 16 B
+      auto issue_o = [&](int w) {
+        const int s = (w >> 8) & 15;
+        const uint64_t va = v_desc + s * (X::TILE >> 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
-            mma_bf16_ss(tm + t * 128, qa + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
-          }
-          mma_commit(&s_full[t]);
-          if (flags & XS_LAST) mma_commit(&q_empty[t]);
-          if (t == 1 && (flags & XS_FREE)) mma_commit(&k_empty[s]);
+        for (int kk = 0; kk < 8; ++kk)
+          mma_bf16_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, va + kk * (2048 >> 4), idesc_o,
+                      kk > 0 || !(w & XS_FIRST) ? 1u : 0u);
+        if (w & XS_LAST) mma_commit(&o_full[t]);
+        if (w & XS_FREE) mma_commit(&v_empty[s]);
+      };
+      // S of step w: 16 columns further are 32 B on within a 64-column half,
+      // BOX on to the next
+      auto issue_s = [&](int w) {
+        const int s = (w >> 8) & 15;
+        const uint64_t ka = k_desc + s * (X::TILE >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+          mma_bf16_ss(tm + t * 128, q_desc + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
         }
-        __syncwarp();
+        mma_commit(&s_full[t]);
+        if (w & XS_LAST) mma_commit(&q_empty[t]);
+        if (w & XS_FREE) mma_commit(&k_empty[s]);
       };
       uint32_t no = 0;
-      // the next step that has products
-      auto next = [&](CrossStep& st) {
-        do {
-          if (!read_step(no, st, rec_ready(no))) return false;
+      // the first word of the next step that has products
+      auto fetch = [&]() {
+        for (;;) {
+          const uint32_t at = no % XT_RECORDS;
+          int w = rec_ready(no) ? records[2 * at].x : XS_END;
+          w = warp_uniform(w);
+          if (lane == 0) mbar_arrive(&rec_empty[at]);
           ++no;
-        } while (st.flags & XS_EMPTY);
-        st.flags = warp_uniform(st.flags);
-        st.load = warp_uniform(st.load);
-        st.item_no = warp_uniform(st.item_no);
-        return true;
+          if (!(w & XS_EMPTY)) return w;
+        }
       };
-      CrossStep cur, nxt;
-      bool have = next(cur);
-      bool ok = have && all(wait(&k_full[cur.load % NS], (cur.load / NS) & 1));
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        ok = ok && all(wait(&q_full[t], 0));
-        tc_fence_after();
-        if (ok) issue_s(t, cur.load % NS, cur.flags);
-      }
-      for (uint32_t step = 0; have && ok; ++step) {
-        const bool more = next(nxt);
-        const int s = cur.load % NS;
-        const uint32_t ph = (cur.load / NS) & 1;
-        ok = wait(&v_full[s], ph) && wait(&aux_full[s], ph);
-        if (more) ok = ok && wait(&k_full[nxt.load % NS], (nxt.load / NS) & 1);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          ok = all(ok && wait(&p_full[t], step & 1));
-          if (!ok) break;
+      // cur: the step whose P comes next, nxt: the step whose S does (XS_END: none)
+      int cur = XS_END, nxt = fetch();
+      uint32_t step = 0;
+      bool ok = true;
+      auto k_ready = [&](int w) { return wait(&k_full[(w >> 8) & 15], (w >> 12) & 1); };
+      while (((cur & nxt) & XS_END) == 0) {
+        // S of the item's next tile goes out behind PV; the first of another
+        // item waits for its queries, which must not hold PV back
+        bool s_due = !(nxt & XS_END);
+        if (!(cur & XS_END)) {  // the side data of a ring slot are ready after its V
+          const bool both = s_due && !(nxt & XS_FIRST);
+          ok = wait(&aux_full[(cur >> 8) & 15], (cur >> 12) & 1) && (!both || k_ready(nxt)) && wait(&p_full[t], step & 1);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          ++step;
           tc_fence_after();
-          // 16 keys further: 16 rows of 128 B; the two 64-column halves are BOX apart (LBO)
-          const uint64_t va = umma_desc_sw128(base + X::OFF_V + s * X::TILE, BOX, 1024);
           if (leader) {
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              mma_bf16_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, va + kk * (2048 >> 4), idesc_o,
-                          kk > 0 || !(cur.flags & XS_FIRST) ? 1u : 0u);
-            if (cur.flags & XS_LAST) mma_commit(&o_full[t]);
-            if (t == 1 && (cur.flags & XS_FREE)) mma_commit(&v_empty[s]);
+            issue_o(cur);
+            if (both) issue_s(nxt);
           }
           __syncwarp();
-          if (more) {
-            if (nxt.flags & XS_FIRST) ok = all(wait(&q_full[t], nxt.item_no & 1));
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(t, nxt.load % NS, nxt.flags);
-          }
+          s_due = s_due && !both;
+        }
+        if (s_due) {
+          ok = k_ready(nxt) && wait(&q_full[t], (nxt >> 13) & 1);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          tc_fence_after();
+          if (leader) issue_s(nxt);
+          __syncwarp();
         }
         cur = nxt;
-        have = more;
+        if (!(cur & XS_END)) nxt = fetch();
       }
-    } else if (warp == 2) {
+    } else {
       // ---------------------------------------- side data of every K/V load
       CrossStep st;
       for (uint32_t no = 0; read_step(no, st, rec_ready(no)); ++no) {
@@ -1006,80 +1059,20 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
           *reinterpret_cast<int*>(aux + 528) = plain ? 0 : 1;
         }
         // V rows of keys that nobody sees
-        const uint32_t lw[4] = {live.x, live.y, live.z, live.w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (!((lw[c] >> lane) & 1u)) {
+        if (~(live.x & live.y & live.z & live.w)) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t lw = c < 2 ? (c ? live.y : live.x) : (c == 2 ? live.z : live.w);
             uint8_t* row = smem + X::OFF_V + s * X::TILE + (32 * c + lane) * 128;
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-              for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(row + h * BOX + 16 * x) = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+            for (int x = 0; x < 8 * HALVES && !((lw >> lane) & 1u); ++x)
+              *reinterpret_cast<uint4*>(row + (x >> 3) * BOX + 16 * (x & 7)) = make_uint4(0, 0, 0, 0);
           }
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&aux_full[s]);
       }
-    } else if (lane == 0) {
-      // -------------------------------------------------------- the walk
-      int range[2];
-      cross_range(P, range);
-      const int per = P.pairs * P.qtiles;
-      int load = 0, item_no = 0, run_base = 0;
-      uint32_t no = 0;
-      auto put = [&](const CrossStep& st) {
-        const uint32_t at = no % XT_RECORDS;
-        if (no >= XT_RECORDS && !mbar_wait_fast(smem_u32(&rec_empty[at]), ((no / XT_RECORDS) & 1) ^ 1, abort_addr, ERR_WAIT_LOAD)) return false;
-        records[2 * at] = make_int4(st.flags, st.j, st.load, st.item_no);
-        records[2 * at + 1] = make_int4(st.b, st.hk, st.h0, st.q0);
-        mbar_arrive(&rec_full[at]);
-        ++no;
-        return true;
-      };
-      bool ok = true;
-      CrossStep st;
-      for (int i = range[0]; i < range[1] && ok; ++i) {
-        const int key = i / per, rem = i % per;
-        const int pair = rem / P.qtiles, qt = rem % P.qtiles;
-        st.b = key / p.kvheads;
-        st.hk = key % p.kvheads;
-        st.h0 = st.hk * p.group + (P.qpair ? pair : 2 * pair);
-        st.q0 = qt * (P.qpair ? 2 * XT_BM : XT_BM);
-        const int tiles = (cross_keys(p, st.b) + XT_BN - 1) / XT_BN;
-        const bool run_first = i == range[0] || rem == 0, run_last = i == range[1] - 1 || rem == per - 1;
-        // K and V of a run of items stay when all their tiles fit the ring
-        // (not under a packed mask: which V rows are zeroed depends on the item)
-        const bool resident = !P.bits && tiles <= NS;
-        if (resident && run_first) run_base = load, load += tiles;
-        auto next_tile = [&](int j) {
-          if (P.bits)
-            for (; j < tiles; ++j) {
-              const uint4 w = cross_seen(P, st.b, st.h0, st.q0, j);
-              if (w.x | w.y | w.z | w.w) break;
-            }
-          return j;
-        };
-        st.j = next_tile(0);
-        st.item_no = item_no;
-        if (st.j >= tiles) {
-          st.flags = XS_FIRST | XS_LAST | XS_EMPTY;
-          st.load = 0;
-          ok = put(st);
-          continue;
-        }
-        ++item_no;
-        for (int j = st.j, first = 1; j < tiles && ok; first = 0) {
-          const int after = next_tile(j + 1);
-          st.j = j;
-          st.load = resident ? run_base + j : load++;
-          st.flags = (first ? XS_FIRST : 0) | (after >= tiles ? XS_LAST : 0) | (!resident || run_first ? XS_LOAD : 0) |
-                     (!resident || run_last ? XS_FREE : 0);
-          ok = put(st);
-          j = after;
-        }
-      }
-      st.flags = XS_END;
-      if (ok) put(st);
     }
   }
 
@@ -1092,9 +1085,9 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
       for (int x = max(0, k_loads - NS); x < k_loads; ++x) mbar_drain(&k_full[x % NS], (x / NS) & 1);
       for (int x = max(0, v_loads - NS); x < v_loads; ++x) mbar_drain(&v_full[x % NS], (x / NS) & 1);
     }
-    if (warp == 1 && leader) {  // behind every product issued
-      mma_commit(drained);
-      mbar_drain(drained, 0);
+    if ((warp == 1 || warp == 3) && leader) {  // behind every product issued
+      mma_commit(drained + (warp >> 1));
+      mbar_drain(drained + (warp >> 1), 0);
     }
     __syncwarp();
   }
