@@ -463,16 +463,24 @@ static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void*
 }
 
 // --------------------------------------------------------- qk_norm_rope
-static int qk_norm_rope_launch(QkNormParams p, int dim, int dtype, cudaStream_t st) {
-  const long long items = p.side[0].items + p.side[1].items;
-  const long long grid = (items + QKN_THREADS / 32 - 1) / (QKN_THREADS / 32);
-  if (grid > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+static int qk_norm_rope_launch(const QkNormParams& p, int dim, int dtype, cudaStream_t st) {
   typedef void (*Kernel)(QkNormParams);
-  const Kernel kern = dtype == COND_BF16 ? (dim == 128 ? (Kernel)qk_norm_rope_kernel<__nv_bfloat16, 128>
-                                                       : (Kernel)qk_norm_rope_kernel<__nv_bfloat16, 64>)
-                                         : (dim == 128 ? (Kernel)qk_norm_rope_kernel<__half, 128>
-                                                       : (Kernel)qk_norm_rope_kernel<__half, 64>);
-  kern<<<(unsigned)grid, QKN_THREADS, 0, st>>>(p);
+  static const Kernel kernels[2][2] = {
+      {qk_norm_rope_kernel<__nv_bfloat16, 128>, qk_norm_rope_kernel<__nv_bfloat16, 64>},
+      {qk_norm_rope_kernel<__half, 128>, qk_norm_rope_kernel<__half, 64>}};
+  const int ti = dtype == COND_BF16 ? 0 : 1, di = dim == 128 ? 0 : 1;
+  static int resident[64][4];
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  int& wave = resident[dev][2 * ti + di];
+  if (wave == 0) {
+    rc = resident_blocks(kernels[ti][di], QKN_THREADS, 0, &wave);
+    if (rc) return rc;
+  }
+  const uint32_t items = p.side[0].items + p.side[1].items;
+  const uint32_t blocks = (items + QKN_THREADS / 32 - 1) / (QKN_THREADS / 32);
+  kernels[ti][di]<<<blocks < (uint32_t)wave ? blocks : wave, QKN_THREADS, 0, st>>>(p);
   return launch_status();
 }
 
@@ -928,7 +936,7 @@ K2B_EXPORT int k2b_w4_linear(const void* x, long long x_stride, const void* pack
   W4Params p;
   memset(&p, 0, sizeof(p));
   p.w = static_cast<const uint8_t*>(packed);
-  p.scales = static_cast<const __half*>(scales);
+  p.scales = static_cast<const unsigned short*>(scales);
   p.bias = bias;
   p.out = out;
   p.m = m;
@@ -948,11 +956,14 @@ K2B_EXPORT int k2b_qk_norm_rope(const void* q, const void* k, const void* wq, co
       (dtype != COND_FP16 && dtype != COND_BF16) || (fq && fq_batch != 1 && fq_batch != batch) ||
       (fk && fk_batch != 1 && fk_batch != batch))
     return (int)cudaErrorInvalidValue;
+  const int qc = (heads + QKN_HEADS - 1) / QKN_HEADS, kc = (kvheads + QKN_HEADS - 1) / QKN_HEADS;
+  const long long qi = (long long)batch * lq * qc, ki = (long long)batch * lk * kc;
+  if (qi + ki > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   QkNormParams p;
   p.side[0] = {q, qo, static_cast<const float*>(wq), static_cast<const float*>(fq), q_sb, q_sh, q_st, lq, heads,
-               fq_batch, eps_q, (long long)batch * lq * ((heads + QKN_HEADS - 1) / QKN_HEADS)};
+               fq_batch, eps_q, qc, (uint32_t)qi};
   p.side[1] = {k, ko, static_cast<const float*>(wk), static_cast<const float*>(fk), k_sb, k_sh, k_st, lk, kvheads,
-               fk_batch, eps_k, (long long)batch * lk * ((kvheads + QKN_HEADS - 1) / QKN_HEADS)};
+               fk_batch, eps_k, kc, (uint32_t)ki};
   for (const QkNormSide& s : p.side) {
     if (s.length == 0) continue;
     if (!s.x || !s.y || !s.w || !aligned16(s.x) || !aligned16(s.y) || !aligned16(s.w) || !aligned16(s.freqs) ||

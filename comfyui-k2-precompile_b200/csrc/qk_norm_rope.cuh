@@ -10,10 +10,11 @@
 //
 // Bound by memory: 2 bytes read and 2 written per value, plus 8 D bytes of
 // table per token.  D/8 lanes own a head (16 bytes each), so a warp takes
-// 256 values at once; a warp's item is one token and QKN_HEADS heads, whose
-// loads are all in flight before the first is used, and which share the
-// token's table entries in registers.  The items of a token are neighbours,
-// so the table comes from L1 after the first.
+// 256 values at once; a warp's item is one token and QKN_HEADS heads.  The
+// warps of a resident wave walk over the items, and a warp loads its next item
+// before it works on the present one, so that loads are always in flight.  The
+// items of a token are neighbours: its table entries come from L1 after the
+// first, and w + 1 is folded into them once per item.
 #pragma once
 #include "elem16.cuh"
 
@@ -30,77 +31,120 @@ struct QkNormSide {
   long long sb, sh, st;
   int length, heads, fb;
   float eps;
-  long long items;    // batch * length * ceil(heads / QKN_HEADS)
+  int chunks;         // ceil(heads / QKN_HEADS)
+  uint32_t items;     // batch * length * chunks
 };
 struct QkNormParams {
   QkNormSide side[2];
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(QKN_THREADS) qk_norm_rope_kernel(const __grid_constant__ QkNormParams p) {
+__global__ void __launch_bounds__(QKN_THREADS, 3) qk_norm_rope_kernel(const __grid_constant__ QkNormParams p) {
   constexpr int LPH = D / 8;               // lanes per head
   constexpr int HPS = 32 / LPH;            // heads per step
   constexpr int STEPS = QKN_HEADS / HPS;
   const int lane = threadIdx.x & 31;
-  long long item = (long long)blockIdx.x * (QKN_THREADS / 32) + (threadIdx.x >> 5);
-  const bool second = item >= p.side[0].items;
-  if (second) item -= p.side[0].items;
-  const QkNormSide& s = p.side[second ? 1 : 0];
-  if (item >= s.items) return;
-  const int chunks = (s.heads + QKN_HEADS - 1) / QKN_HEADS;
-  const long long row = item / chunks;     // batch * length + token
-  const int h0 = (int)(item % chunks) * QKN_HEADS + lane / LPH;
-  const long long b = row / s.length, tok = row % s.length;
   const int c = (lane % LPH) * 8;          // this lane's first column
+  const uint32_t total = p.side[0].items + p.side[1].items;
+  const uint32_t stride = gridDim.x * (QKN_THREADS / 32);
 
-  const T* x = static_cast<const T*>(s.x) + b * s.sb + tok * s.st + c;
+  struct Item {
+    int side, h0;
+    uint32_t b, tok;
+  };
+  auto locate = [&](uint32_t i) {
+    Item it;
+    it.side = i >= p.side[0].items;
+    const QkNormSide& s = p.side[it.side];
+    if (it.side) i -= p.side[0].items;
+    const uint32_t row = i / s.chunks;     // batch * length + token
+    it.h0 = (int)(i - row * s.chunks) * QKN_HEADS + lane / LPH;
+    it.b = row / s.length;
+    it.tok = row - it.b * s.length;
+    return it;
+  };
+  auto load = [&](const Item& it, uint4 (&v)[STEPS]) {
+    const QkNormSide& s = p.side[it.side];
+    const T* x = static_cast<const T*>(s.x) + it.b * s.sb + it.tok * s.st + c;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+      if (it.h0 + i * HPS < s.heads) v[i] = ldg_stream(x + (long long)(it.h0 + i * HPS) * s.sh);
+  };
+
+  uint32_t at = blockIdx.x * (QKN_THREADS / 32) + (threadIdx.x >> 5);
+  if (at >= total) return;
+  Item it = locate(at);
   uint4 v[STEPS];
+  load(it, v);
+  for (;;) {
+    const uint32_t next = at + stride;
+    const bool more = next < total && next > at;
+    Item nit = it;
+    uint4 nv[STEPS];
+    if (more) {
+      nit = locate(next);
+      load(nit, nv);
+    }
+    const QkNormSide& s = p.side[it.side];
+    // f[4 j ..]: the pair's matrix with the norm weights of its columns, or the weights alone
+    float f[16];
+    {
+      float w[8];
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i)
-    if (h0 + i * HPS < s.heads) v[i] = ldg_stream(x + (long long)(h0 + i * HPS) * s.sh);
-  float w[8], f[16];
+      for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4*>(w + i) = __ldg(reinterpret_cast<const float4*>(s.w + c + i));
+      if (s.freqs) {
+        const float* fr = s.freqs + ((long long)(s.fb == 1 ? 0 : it.b) * s.length + it.tok) * (2 * D) + 2 * c;
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4*>(w + i) = __ldg(reinterpret_cast<const float4*>(s.w + c + i));
-  if (s.freqs) {
-    const float* fr = s.freqs + ((s.fb == 1 ? 0 : b) * s.length + tok) * (2 * D) + 2 * c;
+        for (int i = 0; i < 16; i += 4) {
+          const float4 m = __ldg(reinterpret_cast<const float4*>(fr + i));
+          const float w0 = w[i / 2] + 1.0f, w1 = w[i / 2 + 1] + 1.0f;
+          f[i] = m.x * w0, f[i + 1] = m.y * w1, f[i + 2] = m.z * w0, f[i + 3] = m.w * w1;
+        }
+      } else {
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(f + i) = __ldg(reinterpret_cast<const float4*>(fr + i));
-  }
+        for (int i = 0; i < 16; i += 4) {
+          f[i] = w[i / 2] + 1.0f, f[i + 3] = w[i / 2 + 1] + 1.0f;
+          f[i + 1] = f[i + 2] = 0.0f;
+        }
+      }
+    }
+    const bool turn = s.freqs != nullptr;
+    T* y = static_cast<T*>(s.y) + (((long long)it.b * s.length + it.tok) * s.heads) * D + c;
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int h = h0 + i * HPS;
-    const bool live = h < s.heads;
-    float e[8];
-    float sum = 0.0f;
-    if (live) {
-      const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    for (int i = 0; i < STEPS; ++i) {
+      const int h = it.h0 + i * HPS;
+      const bool live = h < s.heads;
+      float e[8];
+      float sum = 0.0f;
+      if (live) {
+        const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 a = Elem16<T>::unpack(u[j]);
+          e[2 * j] = a.x;
+          e[2 * j + 1] = a.y;
+          sum = fmaf(a.x, a.x, fmaf(a.y, a.y, sum));
+        }
+      }
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (!live) continue;
+      const float r = rsqrtf(sum * (1.0f / D) + s.eps);
+      uint32_t o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 a = Elem16<T>::unpack(u[j]);
-        e[2 * j] = a.x;
-        e[2 * j + 1] = a.y;
-        sum = fmaf(a.x, a.x, fmaf(a.y, a.y, sum));
+        const float a = e[2 * j] * r, z = e[2 * j + 1] * r;
+        // (without a table the other column must not enter: 0 * inf)
+        o[j] = turn ? Elem16<T>::pack(fmaf(f[4 * j], a, f[4 * j + 1] * z), fmaf(f[4 * j + 2], a, f[4 * j + 3] * z))
+                    : Elem16<T>::pack(f[4 * j] * a, f[4 * j + 3] * z);
       }
+      *reinterpret_cast<uint4*>(y + (long long)h * D) = make_uint4(o[0], o[1], o[2], o[3]);
     }
+    if (!more) break;
+    at = next;
+    it = nit;
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (!live) continue;
-    const float r = rsqrtf(sum * (1.0f / D) + s.eps);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = e[j] * r * (w[j] + 1.0f);
-    uint32_t o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float a = e[2 * j], z = e[2 * j + 1];
-      if (s.freqs) {
-        const float a1 = fmaf(f[4 * j], a, f[4 * j + 1] * z), z1 = fmaf(f[4 * j + 2], a, f[4 * j + 3] * z);
-        a = a1;
-        z = z1;
-      }
-      o[j] = Elem16<T>::pack(a, z);
-    }
-    T* y = static_cast<T*>(s.y) + (row * s.heads + h) * D + c;
-    *reinterpret_cast<uint4*>(y) = make_uint4(o[0], o[1], o[2], o[3]);
+    for (int i = 0; i < STEPS; ++i) v[i] = nv[i];
   }
 }
 

@@ -124,7 +124,7 @@ __device__ __forceinline__ float w4_act(float y, int act) {
 
 struct W4Params {
   const uint8_t* w;      // [n, k/2]
-  const __half* scales;  // [n, groups]
+  const unsigned short* scales;  // fp16 [n, groups]
   const uint8_t* frag;   // prepared rows
   const float* factor;
   const void* bias;      // [n] or null
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(W4_THREADS) w4_linear_kernel(const __grid_cons
 
   struct Item {
     uint4 a, b;
-    __half sa, sb;
+    uint32_t sa, sb;  // fp16 scales, a register each: packed in one they would be merged, and waited for, at the load
   };
   Item buf[W4_DEPTH];
   // the next item to load
@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(W4_THREADS) w4_linear_kernel(const __grid_cons
               mma16816<__half>(c[i], ha[2], hb[2], ha[3], hb[3], xv.z, xv.w);
             }
           }
-          const float sa = __half2float(buf[s].sa), sb = __half2float(buf[s].sb);
+          const float sa = __half2float(__ushort_as_half((unsigned short)buf[s].sa));
+          const float sb = __half2float(__ushort_as_half((unsigned short)buf[s].sb));
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
             const long long at = (long long)min(block0 + i, mblocks - 1) * p.groups + g;
