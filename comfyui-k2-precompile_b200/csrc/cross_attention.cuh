@@ -49,6 +49,7 @@ constexpr int XF_THREADS = 256;
 constexpr int XF_WARPS = XF_THREADS / 32;
 constexpr int XF_ROWS = 16;
 constexpr int XF_KEYS = 16;
+constexpr int XF_SPLITS = 8;  // CTAs of a cluster at most
 
 template <int D>
 constexpr int xf_smem_bytes() {
@@ -67,8 +68,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// CTAs per SM: two at D = 64 (within 128 registers), one at D = 128 (219).
+__host__ __device__ constexpr int xf_per_sm(int dim) { return dim == 64 ? 2 : 1; }
+
 template <typename T, int D>
-__global__ void __launch_bounds__(XF_THREADS) cross_few_kernel(const __grid_constant__ CrossParams p) {
+__global__ void __launch_bounds__(XF_THREADS, D == 64 ? xf_per_sm(64) : 0) cross_few_kernel(const __grid_constant__ CrossParams p) {
   extern __shared__ float xf_smem[];
   float* so = xf_smem;                            // [warps][16][D]
   float* sred = so + XF_WARPS * XF_ROWS * D;      // [16][D]
@@ -132,7 +136,9 @@ __global__ void __launch_bounds__(XF_THREADS) cross_few_kernel(const __grid_cons
   if (tile < tiles) load_k(tile);
   for (; tile < tiles; tile += stride) {
     const int k0 = tile * XF_KEYS;
-    // V of keys 2t, 2t + 1, 2t + 8, 2t + 9; columns 64 e + 8 r..
+    // V of keys 2t, 2t + 1, 2t + 8, 2t + 9; columns 64 e + 8 r..  (Loaded an
+    // iteration earlier, behind the PV of the last, it measured slower: one
+    // query by 4096 keys of 12 heads 17.0 against 13.8 us.)
     uint4 vf[4][D / 64];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -293,13 +299,24 @@ __global__ void __launch_bounds__(XF_THREADS) cross_few_kernel(const __grid_cons
       sum = sml[XF_ROWS + row];
       val = sred[at];
     } else {
-      for (int c = 0; c < p.splits; ++c)
-        top = fmaxf(top, ld_cluster_f32(cluster_map(smem_u32(sml + row), c)));
-      for (int c = 0; c < p.splits; ++c) {
-        const float mc = ld_cluster_f32(cluster_map(smem_u32(sml + row), c));
-        const float f = mc == -INFINITY ? 0.0f : exp2_fast((mc - top) * kLog2e);
-        sum = fmaf(ld_cluster_f32(cluster_map(smem_u32(sml + XF_ROWS + row), c)), f, sum);
-        val = fmaf(ld_cluster_f32(cluster_map(smem_u32(sred + at), c)), f, val);
+      // everything in flight before the first is used
+      float mc[XF_SPLITS], lc[XF_SPLITS], vc[XF_SPLITS];
+#pragma unroll
+      for (int c = 0; c < XF_SPLITS; ++c) {
+        mc[c] = -INFINITY, lc[c] = vc[c] = 0.0f;
+        if (c < p.splits) {
+          mc[c] = ld_cluster_f32(cluster_map(smem_u32(sml + row), c));
+          lc[c] = ld_cluster_f32(cluster_map(smem_u32(sml + XF_ROWS + row), c));
+          vc[c] = ld_cluster_f32(cluster_map(smem_u32(sred + at), c));
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < XF_SPLITS; ++c) top = fmaxf(top, mc[c]);
+#pragma unroll
+      for (int c = 0; c < XF_SPLITS; ++c) {
+        const float f = mc[c] == -INFINITY ? 0.0f : exp2_fast((mc[c] - top) * kLog2e);
+        sum = fmaf(lc[c], f, sum);
+        val = fmaf(vc[c], f, val);
       }
     }
     if (rr < rows) {
@@ -363,7 +380,8 @@ struct XtShape {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + 2 * TILE;
   static constexpr int OFF_V = OFF_K + STAGES * TILE;
-  static constexpr int OFF_AUX = OFF_V + STAGES * TILE;
+  static constexpr int OFF_O = OFF_V + STAGES * TILE;  // 4 KB per softmax warp
+  static constexpr int OFF_AUX = OFF_O + 8 * 4096;
   static constexpr int AUX = 128 * 4 + 32;             // addends, keep words, flags
   static constexpr int OFF_REC = OFF_AUX + STAGES * AUX;
   static constexpr int OFF_BAR = OFF_REC + XT_RECORDS * 32;
@@ -399,17 +417,30 @@ __global__ void __launch_bounds__(256)
   const int b = blockIdx.y / mh, h = blockIdx.y % mh;
   uint32_t seen[4] = {0, 0, 0, 0};
   const uint8_t* base = mask + b * m_sb + h * m_sh;
-  for (int i = warp; i < 128; i += 8) {
-    const int row = qt * 128 + i;
-    if (row >= mq) break;
-    uint32_t w[4];
+  const int key0 = kt * 128 + lane;
+  for (int i0 = 0; i0 < 16; i0 += 4) {  // 16 rows per warp, the loads of four in flight
+    bool on[4][4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int key = kt * 128 + 32 * c + lane;
-      w[c] = __ballot_sync(0xffffffffu, key < lk && __ldg(base + row * m_sq + key * m_sk) != 0);
-      seen[c] |= w[c];
+    for (int i = 0; i < 4; ++i) {
+      const int row = qt * 128 + warp * 16 + i0 + i;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int key = key0 + 32 * c;
+        on[i][c] = row < mq && key < lk && __ldg(base + row * m_sq + key * m_sk) != 0;
+      }
     }
-    if (lane == 0) bits[((long long)blockIdx.y * mq + row) * nkt + kt] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = qt * 128 + warp * 16 + i0 + i;
+      uint32_t w[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        w[c] = __ballot_sync(0xffffffffu, on[i][c]);
+        seen[c] |= w[c];
+      }
+      if (lane == 0 && row < mq)
+        bits[((long long)blockIdx.y * mq + row) * nkt + kt] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
   if (lane < 4) any[warp][lane] = lane == 0 ? seen[0] : lane == 1 ? seen[1] : lane == 2 ? seen[2] : seen[3];
   __syncthreads();
@@ -492,13 +523,6 @@ __device__ __forceinline__ uint32_t elect_lane() {
 }
 __device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
-// 32 bytes, a whole sector per lane.
-__device__ __forceinline__ void st_global_32b(void* p, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-
 __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   float2 d;
   asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tadd.rn.f32x2 rd, ra, "
@@ -571,18 +595,21 @@ __device__ __forceinline__ void tmem_ld_row(uint32_t taddr, uint32_t (&r)[64]) {
       : "r"(taddr)
       : "memory");
 }
-// 32 columns of this lane's row, complete on return.
-__device__ __forceinline__ void tmem_ld_row(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st_row(uint32_t taddr, const uint32_t (&r)[64]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      :
-        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
+      "tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, "
+      "%34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, "
+      "%54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64};"
+      ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(r[32]), "r"(r[33]), "r"(r[34]), "r"(r[35]),
+        "r"(r[36]), "r"(r[37]), "r"(r[38]), "r"(r[39]), "r"(r[40]), "r"(r[41]), "r"(r[42]), "r"(r[43]), "r"(r[44]),
+        "r"(r[45]), "r"(r[46]), "r"(r[47]), "r"(r[48]), "r"(r[49]), "r"(r[50]), "r"(r[51]), "r"(r[52]), "r"(r[53]),
+        "r"(r[54]), "r"(r[55]), "r"(r[56]), "r"(r[57]), "r"(r[58]), "r"(r[59]), "r"(r[60]), "r"(r[61]), "r"(r[62]),
+        "r"(r[63])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_row(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -724,30 +751,30 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
         }
         const bool adds = *reinterpret_cast<const int*>(aux + 528) != 0;
         // Scores in log2 units are S * cm.  With addends they replace S first, in
-        // a rolled loop: unrolled it costs the main path its registers, and a
-        // spill here goes to L2 (shared memory leaves L1 next to nothing).
+        // a rolled loop: unrolled it costs the main path registers, and a spill
+        // here goes to L2 (shared memory leaves L1 next to nothing).
         float cm = c;
-        if (adds) {
+        if (__builtin_expect(adds, 0)) {
           cm = 1.0f;
 #pragma unroll 1
-          for (int cc = 0; cc < 4; ++cc) {
-            uint32_t u[32];
-            tmem_ld_row(s_at + 32 * cc, u);
+          for (int cc = 0; cc < 2; ++cc) {
+            uint32_t u[64];
+            tmem_ld_row(s_at + 64 * cc, u);
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 a = *reinterpret_cast<const float4*>(aux + 4 * (32 * cc + e));
+            for (int e = 0; e < 64; e += 4) {
+              const float4 a = *reinterpret_cast<const float4*>(aux + 4 * (64 * cc + e));
               u[e] = __float_as_uint(fmaf(__uint_as_float(u[e]), c, a.x));
               u[e + 1] = __float_as_uint(fmaf(__uint_as_float(u[e + 1]), c, a.y));
               u[e + 2] = __float_as_uint(fmaf(__uint_as_float(u[e + 2]), c, a.z));
               u[e + 3] = __float_as_uint(fmaf(__uint_as_float(u[e + 3]), c, a.w));
             }
-            tmem_st_row(s_at + 32 * cc, u);
+            tmem_st_row(s_at + 64 * cc, u);
           }
           tmem_wait_st();
         }
         uint32_t u[128];
         tmem_ld_row(s_at, u);
-        if (__any_sync(0xffffffffu, (mine.x & mine.y & mine.z & mine.w) != ~0u)) {
+        if (__builtin_expect(__any_sync(0xffffffffu, (mine.x & mine.y & mine.z & mine.w) != ~0u), 0)) {
           const uint32_t mw[4] = {mine.x, mine.y, mine.z, mine.w};
 #pragma unroll
           for (int e = 0; e < 128; ++e)
@@ -819,19 +846,33 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
       // a row that saw no key is zero (its sum is 0, never NaN)
       const bool empty = l_run == 0.0f;
       const float inv = 1.0f / l_run;
-      T* dst = static_cast<T*>(p.out) + (((long long)st.b * p.lq + tok) * p.heads + head) * D;
+      // 64 columns at a time through 4 KB of the warp's own, so that a store
+      // writes four whole 128-byte lines (straight from the rows each wrote 32
+      // sectors of 32 lines, and the output took as long as the tile)
+      uint8_t* stage = smem + X::OFF_O + (warp - 4) * 4096;
+      T* dst = static_cast<T*>(p.out) + (((long long)st.b * p.lq + st.q0 + t * qstep + 32 * w4) * p.heads + head) * D;
+      const int left = p.lq - (st.q0 + t * qstep + 32 * w4);  // rows of this warp that exist
 #pragma unroll 1
       for (int cc = 0; cc < D / 64; ++cc) {
         uint32_t u[64];
         tmem_ld_row(o_at + 64 * cc, u);  // (of an item without keys: not used)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t o[8];
+        for (int x = 0; x < 8; ++x) {
+          uint32_t o[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            o[e] = empty ? 0u : Elem16<T>::pack(__uint_as_float(u[16 * x + 2 * e]) * inv, __uint_as_float(u[16 * x + 2 * e + 1]) * inv);
-          if (tok < p.lq) st_global_32b(dst + 64 * cc + 16 * x, o);
+          for (int e = 0; e < 4; ++e)
+            o[e] = empty ? 0u : Elem16<T>::pack(__uint_as_float(u[8 * x + 2 * e]) * inv, __uint_as_float(u[8 * x + 2 * e + 1]) * inv);
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((x ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int row = 4 * x + (lane >> 3), chunk = lane & 7;
+          const uint4 o = *reinterpret_cast<const uint4*>(stage + row * 128 + ((chunk ^ (row & 7)) << 4));
+          if (row < left)
+            *reinterpret_cast<uint4*>(dst + (long long)row * p.heads * D + 64 * cc + 8 * chunk) = o;
+        }
+        __syncwarp();
       }
     }
   } else {

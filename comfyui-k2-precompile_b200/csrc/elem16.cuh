@@ -37,12 +37,21 @@ struct Elem16<__half> {
   static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 };
 
-// 16 bytes that this kernel reads once: not kept in L1.
+// 16 bytes that this kernel reads once: not kept in L1, and fetched with their
+// neighbours into L2 (rows of 64 bytes at a time are what these kernels ask for).
 __device__ __forceinline__ uint4 ldg_stream(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
+  return v;
+}
+
+// A 16-bit value loaded ahead of its use: volatile, so that the compiler does
+// not move the load down to the use to save the register.
+__device__ __forceinline__ uint32_t ldg_ahead_u16(const void* p) {
+  unsigned short v;
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
   return v;
 }
 

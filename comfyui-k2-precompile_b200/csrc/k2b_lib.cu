@@ -429,29 +429,25 @@ static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void*
   if (rc) return rc;
   p.frag = frag;
   p.factor = factor;
-  // warps along k: as many as there are groups for
-  p.kw = p.groups >= 8 ? 8 : p.groups >= 4 ? 4 : p.groups >= 2 ? 2 : 1;
-  // activation blocks per CTA: every block of the rows while they fit the accumulators
+  // Warps along k: one per row tile where the tiles alone give every SM its
+  // sixteen warps, else as many as it takes (a warp keeps at least two groups).
+  const long long row_tiles = (p.n + 15) / 16;
   const int sel = mblocks == 1 ? 0 : mblocks == 2 ? 1 : 2;
-  const int nt = 1 << sel;
-  typedef void (*Kernel)(W4Params);
-  static const Kernel kernels[3] = {w4_linear_kernel<T, 1>, w4_linear_kernel<T, 2>, w4_linear_kernel<T, 4>};
-  static int resident[64][3];
-  int dev = 0;
+  const int nt = 1 << sel, gy = (mblocks + nt - 1) / nt;
+  int sms = 0, dev = 0;
   rc = current_device(&dev);
   if (rc) return rc;
-  if (resident[dev][sel] == 0) {
-    rc = resident_blocks(kernels[sel], W4_THREADS, 0, &resident[dev][sel]);
-    if (rc) return rc;
-  }
+  cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return (int)e;
+  p.kw = 1;
+  while (p.kw < W4_WARPS && p.groups >= 4 * p.kw && row_tiles * gy * p.kw < 15LL * sms) p.kw *= 2;
+  if (gy > 65535) return (int)cudaErrorInvalidValue;
+  typedef void (*Kernel)(W4Params);
+  static const Kernel kernels[3] = {w4_linear_kernel<T, 1>, w4_linear_kernel<T, 2>, w4_linear_kernel<T, 4>};
   const int rows_per_cta = 16 * (W4_WARPS / p.kw);
-  const int tiles = (p.n + rows_per_cta - 1) / rows_per_cta;
-  const int gy = (mblocks + nt - 1) / nt;
-  int gx = resident[dev][sel] / gy;
-  gx = gx < 1 ? 1 : gx > tiles ? tiles : gx;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(gx, gy, 1);
+  cfg.gridDim = dim3((p.n + rows_per_cta - 1) / rows_per_cta, gy, 1);
   cfg.blockDim = dim3(W4_THREADS, 1, 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -485,6 +481,23 @@ static int qk_norm_rope_launch(const QkNormParams& p, int dim, int dtype, cudaSt
 }
 
 // ------------------------------------------------------ cross attention
+// SMs of a B200; only balance and the choice of kernel depend on it.
+constexpr int kSms = 148;
+
+static long long cross_few_row_tiles(const CrossParams& p) {
+  return ((long long)p.group * p.lq + XF_ROWS - 1) / XF_ROWS;
+}
+// CTAs that share the keys of a row tile: a cluster, while that gives idle SMs
+// work and every warp of it keeps a tile of keys.
+static int cross_few_splits(const CrossParams& p, int dim) {
+  const long long ctas = cross_few_row_tiles(p) * p.kvheads * p.batch;
+  int splits = 1;
+  while (splits < XF_SPLITS && ctas * splits * 2 <= xf_per_sm(dim) * kSms &&
+         (long long)splits * 2 * XF_WARPS * XF_KEYS <= p.lk)
+    splits *= 2;
+  return splits;
+}
+
 static int cross_few_launch(CrossParams p, int dim, int dtype, cudaStream_t st) {
   typedef void (*Kernel)(CrossParams);
   static const Kernel kernels[2][2] = {{cross_few_kernel<__nv_bfloat16, 128>, cross_few_kernel<__nv_bfloat16, 64>},
@@ -501,11 +514,9 @@ static int cross_few_launch(CrossParams p, int dim, int dtype, cudaStream_t st) 
     if (e != cudaSuccess) return (int)e;
     attr_set[dev][2 * ti + di] = true;
   }
-  const long long row_tiles = ((long long)p.group * p.lq + XF_ROWS - 1) / XF_ROWS;
+  const long long row_tiles = cross_few_row_tiles(p);
   const long long ctas = row_tiles * p.kvheads * p.batch;
-  // spread the keys over a cluster while that gives idle SMs work and every warp a tile
-  int splits = 1;
-  while (splits < 8 && ctas * splits * 2 <= 148 && (long long)splits * 2 * XF_WARPS * XF_KEYS <= p.lk) splits *= 2;
+  const int splits = cross_few_splits(p, dim);
   if (ctas * splits > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   p.row_tiles = (int)row_tiles;
   p.splits = splits;
@@ -525,15 +536,29 @@ static int cross_few_launch(CrossParams p, int dim, int dtype, cudaStream_t st) 
   return (int)cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-// Which kernel takes the call: tiles of 128 queries from XT_MIN_QUERIES on.
-// Below, most rows of a tile would be empty.  A negative or zero scale and
-// axes with stride 0 (other than a shared batch of K and V) also take the
-// other kernel: the tile kernel's row maximum is that of q k^T, and a tensor
-// map has no stride 0.
-constexpr int XT_MIN_QUERIES = 33;
-static bool cross_takes_tiles(const CrossParams& p) {
-  return p.lq >= XT_MIN_QUERIES && p.lk > 0 && p.scale > 0.0f && p.q_sb > 0 && p.q_sh > 0 && p.q_st > 0 && p.k_sh > 0 &&
-         p.k_st > 0 && p.v_sh > 0 && p.v_st > 0 && (p.k_sb == 0) == (p.v_sb == 0);
+// Which kernel takes the call.  Both sides' times in tenths of a microsecond
+// from their numbers of waves, fitted to calls of 1 to 300 queries by 16 to
+// 4096 keys (48/12, 20/20, 8/2 and 5/5 heads, one to eight latents): the few
+// kernel takes about 3.5 us a wave and 1.2 more per 128 keys of a CTA, the
+// tile kernel 2.5 us a round of items and 2.0 per key tile.  Measured, e.g., at
+// 48/12 heads: 32 queries by 700 keys 14 against 21 us, 96 queries 27 against
+// 22; 32 queries by 154 keys of eight latents 47 against 18.
+static bool cross_tiles_pay(const CrossParams& p, int dim) {
+  const long long splits = cross_few_splits(p, dim), per = xf_per_sm(dim) * kSms;
+  const long long few_waves = (cross_few_row_tiles(p) * p.kvheads * p.batch * splits + per - 1) / per;
+  const long long few = 50 + few_waves * (35 + 12 * ((p.lk + 128 * splits - 1) / (128 * splits)));
+  const bool odd = p.group % 2;
+  const long long span = odd ? 2 * XT_BM : XT_BM;
+  const long long items = (long long)(odd ? p.group : p.group / 2) * ((p.lq + span - 1) / span) * p.kvheads * p.batch;
+  const long long tile = 70 + (items + kSms - 1) / kSms * (25 + 20 * ((p.lk + XT_BN - 1) / XT_BN));
+  return tile < few;
+}
+// A negative or zero scale and axes with stride 0 (other than a shared batch
+// of K and V) always take the few kernel: the tile kernel's row maximum is
+// that of q k^T, and a tensor map has no stride 0.
+static bool cross_takes_tiles(const CrossParams& p, int dim) {
+  return p.lk > 0 && p.scale > 0.0f && p.q_sb > 0 && p.q_sh > 0 && p.q_st > 0 && p.k_sh > 0 && p.k_st > 0 &&
+         p.v_sh > 0 && p.v_st > 0 && (p.k_sb == 0) == (p.v_sb == 0) && cross_tiles_pay(p, dim);
 }
 
 struct MaskExtent {
@@ -973,16 +998,17 @@ K2B_EXPORT int k2b_qk_norm_rope(const void* q, const void* k, const void* wq, co
   return qk_norm_rope_launch(p, dim, dtype, (cudaStream_t)stream);
 }
 
-K2B_EXPORT long long k2b_cross_workspace_bytes(int batch, int heads, int lq, int lk, long long m_sb, long long m_sh,
-                                               long long m_sq) {
-  if (batch <= 0 || heads <= 0 || lq <= 0 || lk < 0) return -1;
+K2B_EXPORT long long k2b_cross_workspace_bytes(int batch, int heads, int kvheads, int lq, int lk, int dim,
+                                               long long m_sb, long long m_sh, long long m_sq) {
+  if (batch <= 0 || heads <= 0 || kvheads <= 0 || heads % kvheads || lq <= 0 || lk < 0 || (dim != 64 && dim != 128))
+    return -1;
   CrossParams p;
   memset(&p, 0, sizeof(p));
   static const uint8_t some = 0;
   p.mask = &some;
-  p.batch = batch, p.heads = heads, p.lq = lq, p.lk = lk;
+  p.batch = batch, p.heads = heads, p.kvheads = kvheads, p.group = heads / kvheads, p.lq = lq, p.lk = lk;
   p.m_sb = m_sb, p.m_sh = m_sh, p.m_sq = m_sq;
-  return lq >= XT_MIN_QUERIES ? cross_mask_extent(p).bytes : 0;
+  return lk > 0 && cross_tiles_pay(p, dim) ? cross_mask_extent(p).bytes : 0;
 }
 
 K2B_EXPORT int k2b_cross_attention(const void* q, const void* k, const void* v, const void* lengths, const void* mask,
@@ -994,7 +1020,7 @@ K2B_EXPORT int k2b_cross_attention(const void* q, const void* k, const void* v, 
   if (batch <= 0 || heads <= 0 || kvheads <= 0 || heads % kvheads || lq <= 0 || lk < 0 || (dim != 64 && dim != 128) ||
       (dtype != COND_FP16 && dtype != COND_BF16))
     return (int)cudaErrorInvalidValue;
-  if (!q || !out || !aligned16(q) || reinterpret_cast<uintptr_t>(out) % 32 ||
+  if (!q || !out || !aligned16(q) || !aligned16(out) ||
       (lk > 0 && (!k || !v || !aligned16(k) || !aligned16(v))) ||
       (lengths && reinterpret_cast<uintptr_t>(lengths) % 4) || (bias && reinterpret_cast<uintptr_t>(bias) % 4))
     return (int)cudaErrorInvalidValue;
@@ -1013,7 +1039,7 @@ K2B_EXPORT int k2b_cross_attention(const void* q, const void* k, const void* v, 
   p.v_sb = v_sb, p.v_sh = v_sh, p.v_st = v_st;
   p.m_sb = m_sb, p.m_sh = m_sh, p.m_sq = m_sq, p.m_sk = m_sk, p.bias_sb = bias_sb;
   p.scale = scale;
-  return cross_takes_tiles(p) ? cross_tile_launch(p, workspace, dim, dtype, (cudaStream_t)stream)
+  return cross_takes_tiles(p, dim) ? cross_tile_launch(p, workspace, dim, dtype, (cudaStream_t)stream)
                               : cross_few_launch(p, dim, dtype, (cudaStream_t)stream);
 }
 

@@ -268,7 +268,7 @@ PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                 qi = fits_int(Lq, "cross_attention"), ki = fits_int(Lk, "cross_attention");
       at::Tensor work;
       if (ms[1] || ms[2]) {  // depends on the head or the query: packed to bits first
-        const long long bytes = k2b_cross_workspace_bytes(bi, hi, qi, ki, ms[0], ms[1], ms[2]);
+        const long long bytes = k2b_cross_workspace_bytes(bi, hi, (int)hk.H, qi, ki, (int)hq.D, ms[0], ms[1], ms[2]);
         if (bytes > 0) work = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
       }
       rc = k2b_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(lengths), ptr(mask), ptr(bias),

@@ -18,14 +18,17 @@
 // so it costs a rotated row 2^-12 (a bf16 rounding would cost 2^-9, as much as
 // the output's), and an unrotated bf16 or fp16 row nothing.
 //
-// w4_linear_kernel: a warp takes 16 weight rows (the product's M) and one
-// group of 128 columns at a time, straight from the checkpoint's layout: lane
+// w4_linear_kernel: a warp takes 16 weight rows (the product's M) and a
+// contiguous range of groups, straight from the checkpoint's layout: lane
 // (r, t) loads the 32 codes 32 t.. of rows r and r + 8 with one 16-byte load
 // each.  The k order inside a matrix product is free, so its 8 codes per
 // 32-bit word become two k16 steps without any exchange; x' is laid out for
-// that order by the prepare kernel, one 16-byte load per word.  Codes become
-// fp16 exactly by setting the exponent of 1024 around a nibble.  Each group's
-// sum is scaled by s and the row's power of two in fp32 and added up in fp32.
+// that order by the prepare kernel, one 16-byte load per word, which L1 serves
+// to the CTA's other warps.  Codes become fp16 exactly by setting the exponent
+// of 1024 around a nibble.  Each group's sum is scaled by s and the row's
+// power of two in fp32 and added up in fp32.  Three or five groups of
+// weights and scales are in flight per warp.  Where there are too few row tiles to fill
+// the GPU, up to eight warps share a tile along k and add up in a fixed order.
 #pragma once
 #include "elem16.cuh"
 
@@ -33,7 +36,6 @@ namespace k2b {
 
 constexpr int W4_THREADS = 256;
 constexpr int W4_WARPS = W4_THREADS / 32;
-constexpr int W4_DEPTH = 4;  // groups in flight per warp
 enum W4Act : int { W4_NONE = 0, W4_GELU = 1, W4_SILU = 2 };
 
 // x' of 8 rows and one group: 4 words of 8 columns x 8 rows x 4 column quarters
@@ -135,116 +137,122 @@ struct W4Params {
 
 // NT: blocks of 8 activation rows of this CTA (blockIdx.y * NT first).
 template <typename T, int NT>
-__global__ void __launch_bounds__(W4_THREADS) w4_linear_kernel(const __grid_constant__ W4Params p) {
-  __shared__ float red[2][W4_WARPS][16][8 * NT + 1];
+__global__ void __launch_bounds__(W4_THREADS, 2) w4_linear_kernel(const __grid_constant__ W4Params p) {
+  constexpr int CH = NT == 1 ? 4 : NT == 2 ? 2 : 1;
+  // groups in flight per warp: what leaves registers for two CTAs per SM
+  constexpr int DEPTH = NT == 4 ? 3 : 5;
+  __shared__ float red[W4_WARPS][16][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
   const int kw = p.kw, rw = W4_WARPS / kw;
   const int wk = warp % kw, wr = warp / kw;
-  const int tiles = (p.n + 16 * rw - 1) / (16 * rw);
-  const int per_tile = (p.groups + kw - 1) / kw;
+  const int per = (p.groups + kw - 1) / kw;
+  const int g0 = wk * per, count = min(per, p.groups - g0);  // (may be none)
   const long long row_bytes = (long long)p.groups * 64;
-  const int block0 = blockIdx.y * NT;
-  const int mblocks = (p.m + 7) / 8;
+  const int block0 = blockIdx.y * NT, mblocks = (p.m + 7) / 8;
+  const int n0 = blockIdx.x * 16 * rw;  // the CTA's first weight row
+  const int ra = min(n0 + wr * 16 + r, p.n - 1), rb = min(n0 + wr * 16 + r + 8, p.n - 1);
 
-  struct Item {
-    uint4 a, b;
-    uint32_t sa, sb;  // fp16 scales, a register each: packed in one they would be merged, and waited for, at the load
-  };
-  Item buf[W4_DEPTH];
-  // the next item to load
-  int ltile = blockIdx.x, lj = 0;
-  auto load = [&](Item& it) {
-    const int g = wk + lj * kw;
-    if (ltile < tiles && g < p.groups) {
-      const int n0 = (ltile * rw + wr) * 16 + r;
-      const int ra = min(n0, p.n - 1), rb = min(n0 + 8, p.n - 1);
-      it.a = ldg_stream(p.w + ra * row_bytes + g * 64 + t * 16);
-      it.b = ldg_stream(p.w + rb * row_bytes + g * 64 + t * 16);
-      it.sa = __ldg(p.scales + (long long)ra * p.groups + g);
-      it.sb = __ldg(p.scales + (long long)rb * p.groups + g);
-    }
-    if (++lj == per_tile) {
-      lj = 0;
-      ltile += gridDim.x;
-    }
+  uint4 wa[DEPTH], wb[DEPTH];
+  uint32_t sa[DEPTH], sb[DEPTH];  // fp16 scales, a register each
+  const uint8_t* pa = p.w + ra * row_bytes + g0 * 64 + t * 16;
+  const uint8_t* pb = p.w + rb * row_bytes + g0 * 64 + t * 16;
+  const unsigned short* qa = p.scales + (long long)ra * p.groups + g0;
+  const unsigned short* qb = p.scales + (long long)rb * p.groups + g0;
+  auto load = [&](int s) {
+    wa[s] = ldg_stream(pa + s * 64);
+    wb[s] = ldg_stream(pb + s * 64);
+    sa[s] = ldg_ahead_u16(qa + s);
+    sb[s] = ldg_ahead_u16(qb + s);
   };
 #pragma unroll
-  for (int i = 0; i < W4_DEPTH; ++i) load(buf[i]);
+  for (int s = 0; s < DEPTH; ++s)
+    if (s < count) load(s);
   pdl_wait();
 
+  // x' of row r of each block; rows past m are zero and are not read
+  const uint8_t* px[NT];
+  const float* pf[NT];
+  bool live[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const long long at = (long long)min(block0 + i, mblocks - 1) * p.groups + g0;
+    px[i] = p.frag + at * W4_FRAG_BYTES + lane * 16;
+    pf[i] = p.factor + at * 8 + 2 * t;
+    live[i] = (block0 + i) * 8 + r < p.m;
+  }
   float acc[NT][4];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+  for (int i0 = 0; i0 < count; i0 += DEPTH) {
+    pa += DEPTH * 64;
+    pb += DEPTH * 64;
+    qa += DEPTH;
+    qb += DEPTH;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-  int tile = blockIdx.x, j = 0, parity = 0;
-  while (tile < tiles) {
+    for (int s = 0; s < DEPTH; ++s) {
+      if (i0 + s < count) {
+        const uint32_t ua[4] = {wa[s].x, wa[s].y, wa[s].z, wa[s].w};
+        const uint32_t ub[4] = {wb[s].x, wb[s].y, wb[s].z, wb[s].w};
+        // CH chains of products per block: one of eight would hold the warp up
+        // for 8 x 24 cycles at the scaling below
+        float c[CH][NT][4];
 #pragma unroll
-    for (int s = 0; s < W4_DEPTH; ++s) {
-      if (tile < tiles) {
-        const int g = wk + j * kw;
-        if (g < p.groups) {
-          const uint32_t wa[4] = {buf[s].a.x, buf[s].a.y, buf[s].a.z, buf[s].a.w};
-          const uint32_t wb[4] = {buf[s].b.x, buf[s].b.y, buf[s].b.z, buf[s].b.w};
-          float c[NT][4];
+        for (int i = 0; i < CH * NT; ++i) c[i / NT][i % NT][0] = c[i / NT][i % NT][1] = c[i / NT][i % NT][2] = c[i / NT][i % NT][3] = 0.0f;
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) c[i][q] = 0.0f;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t ha[4], hb[4];
-            w4_codes(wa[w], ha);
-            w4_codes(wb[w], hb);
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              const long long at = (long long)min(block0 + i, mblocks - 1) * p.groups + g;
-              const uint4 xv = *reinterpret_cast<const uint4*>(p.frag + at * W4_FRAG_BYTES + (w * 32 + lane) * 16);
-              mma16816<__half>(c[i], ha[0], hb[0], ha[1], hb[1], xv.x, xv.y);
-              mma16816<__half>(c[i], ha[2], hb[2], ha[3], hb[3], xv.z, xv.w);
-            }
-          }
-          const float sa = __half2float(__ushort_as_half((unsigned short)buf[s].sa));
-          const float sb = __half2float(__ushort_as_half((unsigned short)buf[s].sb));
+        for (int w = 0; w < 4; ++w) {
+          uint32_t ha[4], hb[4];
+          w4_codes(ua[w], ha);
+          w4_codes(ub[w], hb);
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            const long long at = (long long)min(block0 + i, mblocks - 1) * p.groups + g;
-            const float2 f = *reinterpret_cast<const float2*>(p.factor + at * 8 + 2 * t);
-            acc[i][0] = fmaf(c[i][0] * f.x, sa, acc[i][0]);
-            acc[i][1] = fmaf(c[i][1] * f.y, sa, acc[i][1]);
-            acc[i][2] = fmaf(c[i][2] * f.x, sb, acc[i][2]);
-            acc[i][3] = fmaf(c[i][3] * f.y, sb, acc[i][3]);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (live[i]) x = *reinterpret_cast<const uint4*>(px[i] + s * W4_FRAG_BYTES + w * 512);
+            mma16816<__half>(c[w % CH][i], ha[0], hb[0], ha[1], hb[1], x.x, x.y);
+            mma16816<__half>(c[w % CH][i], ha[2], hb[2], ha[3], hb[3], x.z, x.w);
           }
         }
-        load(buf[s]);
-        if (++j == per_tile) {
-          // the tile's sums over the kw warps, in warp order
+        const float fa = __half2float(__ushort_as_half((unsigned short)sa[s]));
+        const float fb = __half2float(__ushort_as_half((unsigned short)sb[s]));
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            red[parity][warp][r][8 * i + 2 * t] = acc[i][0];
-            red[parity][warp][r][8 * i + 2 * t + 1] = acc[i][1];
-            red[parity][warp][r + 8][8 * i + 2 * t] = acc[i][2];
-            red[parity][warp][r + 8][8 * i + 2 * t + 1] = acc[i][3];
-            acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-          }
-          __syncthreads();
-          const int cols = 16 * rw;
-          for (int o = threadIdx.x; o < cols * 8 * NT; o += W4_THREADS) {
-            const int nn = o % cols, xr = o / cols;
-            const int n = tile * cols + nn, row = block0 * 8 + xr;
-            if (n < p.n && row < p.m) {
-              float y = 0.0f;
-              for (int q = 0; q < kw; ++q) y += red[parity][(nn >> 4) * kw + q][nn & 15][xr];
-              if (p.bias) y += Elem16<T>::to_float(static_cast<const T*>(p.bias)[n]);
-              static_cast<T*>(p.out)[(long long)row * p.n + n] = Elem16<T>::from_float(w4_act(y, p.act));
-            }
-          }
-          parity ^= 1;
-          j = 0;
-          tile += gridDim.x;
+        for (int i = 0; i < NT; ++i) {
+          const float2 f = *reinterpret_cast<const float2*>(pf[i] + s * 8);
+#pragma unroll
+          for (int q = 1; q < CH; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[0][i][e] += c[q][i][e];
+          acc[i][0] = fmaf(c[0][i][0] * f.x, fa, acc[i][0]);
+          acc[i][1] = fmaf(c[0][i][1] * f.y, fa, acc[i][1]);
+          acc[i][2] = fmaf(c[0][i][2] * f.x, fb, acc[i][2]);
+          acc[i][3] = fmaf(c[0][i][3] * f.y, fb, acc[i][3]);
         }
+        if (i0 + s + DEPTH < count) load(s);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      px[i] += DEPTH * W4_FRAG_BYTES;
+      pf[i] += DEPTH * 8;
+    }
+  }
+  // the tile's sums over its kw warps, in warp order
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    red[warp][r][8 * i + 2 * t] = acc[i][0];
+    red[warp][r][8 * i + 2 * t + 1] = acc[i][1];
+    red[warp][r + 8][8 * i + 2 * t] = acc[i][2];
+    red[warp][r + 8][8 * i + 2 * t + 1] = acc[i][3];
+  }
+  __syncthreads();
+  const int shift = kw == 8 ? 4 : kw == 4 ? 5 : kw == 2 ? 6 : 7;  // log2 of the CTA's weight rows
+  const int rows = min(8 * NT, p.m - block0 * 8);
+  for (int o = threadIdx.x; o < rows << shift; o += W4_THREADS) {
+    const int nn = o & ((1 << shift) - 1), xr = o >> shift;
+    if (n0 + nn < p.n) {
+      float y = 0.0f;
+      for (int q = 0; q < kw; ++q) y += red[(nn >> 4) * kw + q][nn & 15][xr];
+      if (p.bias) y += Elem16<T>::to_float(static_cast<const T*>(p.bias)[n0 + nn]);
+      static_cast<T*>(p.out)[(long long)(block0 * 8 + xr) * p.n + n0 + nn] = Elem16<T>::from_float(w4_act(y, p.act));
     }
   }
 }

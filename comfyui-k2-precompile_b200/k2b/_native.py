@@ -89,7 +89,7 @@ SIGNATURES = {
     "k2b_w4_workspace_bytes": (_LL, [_I, _I]),
     "k2b_w4_linear": (_I, [_P, _LL] + [_P] * 5 + [_I] * 6 + [_P]),
     "k2b_qk_norm_rope": (_I, [_P] * 8 + [_I] * 6 + [_LL] * 6 + [_I, _I, _F, _F, _I, _P]),
-    "k2b_cross_workspace_bytes": (_LL, [_I] * 4 + [_LL] * 3),
+    "k2b_cross_workspace_bytes": (_LL, [_I] * 6 + [_LL] * 3),
     "k2b_cross_attention": (_I, [_P] * 8 + [_I] * 6 + [_LL] * 14 + [_F, _I, _P]),
     "k2b_expand_e4m3": (_I, [_P, _P, ctypes.c_longlong, _P]),
 }

@@ -225,7 +225,7 @@ int k2b_qk_norm_rope(const void* q, const void* k, const void* wq, const void* w
                      void* qo, void* ko, int batch, int lq, int lk, int heads, int kvheads, int dim, long long q_sb,
                      long long q_sh, long long q_st, long long k_sb, long long k_sh, long long k_st, int fq_batch,
                      int fk_batch, float eps_q, float eps_k, int dtype, void* stream);
-/* out [batch, lq, heads*dim] (32-byte aligned) = softmax(q k^T scale + bias) v
+/* out [batch, lq, heads*dim] (16-byte aligned) = softmax(q k^T scale + bias) v
  * over the keys that are not excluded, 0 for a row without any.  Strides as above; k_sb = v_sb = 0
  * shares K and V among the batch.  Excluded: keys >= lengths[b] (int32 [batch]
  * or null, clamped to 0..lk), keys with bias -inf (fp32 [batch or 1, lk], batch
@@ -233,8 +233,8 @@ int k2b_qk_norm_rope(const void* q, const void* k, const void* wq, const void* w
  * m_sh, m_sq, m_sk, 0 where broadcast, or null).  workspace: the packed form of
  * a mask with m_sh or m_sq, k2b_cross_workspace_bytes bytes on a 16-byte
  * boundary (0 bytes: may be null). */
-long long k2b_cross_workspace_bytes(int batch, int heads, int lq, int lk, long long m_sb, long long m_sh,
-                                    long long m_sq);
+long long k2b_cross_workspace_bytes(int batch, int heads, int kvheads, int lq, int lk, int dim, long long m_sb,
+                                    long long m_sh, long long m_sq);
 int k2b_cross_attention(const void* q, const void* k, const void* v, const void* lengths, const void* mask,
                         const void* bias, void* out, void* workspace, int batch, int heads, int kvheads, int lq, int lk, int dim,
                         long long q_sb, long long q_sh, long long q_st, long long k_sb, long long k_sh,
