@@ -21,7 +21,10 @@ attention at group 1, the gated residuals, SwiGLU + requant), the final
 RMSNorm + modulation is k2b_norm_mod.  The small plain linears around them
 (``first``, the timestep MLP, ``tproj``, ``txtmlp``, ``last.linear``) are
 format-0 projections, which the reference also runs as plain linears
-(native_runtime.cpp:288), here cuBLAS through torch.  The final norm + modulation
+(native_runtime.cpp:288), here cuBLAS through torch -- or, where the weight is an
+``adapter.W4Linear``, this library's few-row INT4 product.  ``weights.adapter``
+adds decoupled cross attention to an encoder's states (an image prompt) in
+front of the blocks.  The final norm + modulation
 is applied to the whole stream and the text rows are dropped afterwards, as
 graph_model.py:296-299 does.
 
@@ -45,6 +48,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .adapter import CrossAdapter, EncoderKeys, W4Linear, synthetic_adapter
 from .model import BlockWeights, Krea2Blocks, ModelConfig, quantize_weight, rope_table, synthetic_blocks
 from .ops import PreparedWeight
 
@@ -90,6 +94,7 @@ class TextBlockWeights:
 
 @dataclass
 class DiTWeights:
+    # plain linears: (weight, bias) bf16, or a W4Linear
     first: Tuple[torch.Tensor, torch.Tensor]     # bf16 [hidden, patch_dim], [hidden]
     tmlp1: Tuple[torch.Tensor, torch.Tensor]     # [hidden, tdim]
     tmlp2: Tuple[torch.Tensor, torch.Tensor]     # [hidden, hidden]
@@ -101,6 +106,15 @@ class DiTWeights:
     last_norm: torch.Tensor                      # fp32 [hidden]
     last: Tuple[torch.Tensor, torch.Tensor]      # [patch_dim, hidden]
     blocks: List[BlockWeights]
+    adapter: Optional[CrossAdapter] = None
+
+
+def _linear(x: torch.Tensor, w, act: str = "none") -> torch.Tensor:
+    """A plain linear of the model, then gelu (tanh form) if asked."""
+    if isinstance(w, W4Linear):
+        return w(x, act)
+    y = F.linear(x, *w)
+    return F.gelu(y, approximate="tanh") if act == "gelu" else y
 
 
 def patchify(x: torch.Tensor, p: int) -> Tuple[torch.Tensor, int, int]:
@@ -184,9 +198,12 @@ class Krea2DiT:
         return self._stacks[key]
 
     def forward(self, x: torch.Tensor, timesteps: torch.Tensor, context: torch.Tensor,
-                trace: Optional[dict] = None) -> torch.Tensor:
+                trace: Optional[dict] = None, image_prompt: Optional[EncoderKeys] = None,
+                strength: float = 1.0) -> torch.Tensor:
         """x bf16 [B, C, H, W] (H, W multiples of the patch), timesteps [B],
-        context bf16 [B, Lt, txtdim] -> bf16 [B, C, H, W].  ``trace``: a dict
+        context bf16 [B, Lt, txtdim] -> bf16 [B, C, H, W].  ``image_prompt``:
+        weights.adapter.keys(...) of an encoder's states, added with
+        ``strength``.  ``trace``: a dict
         that receives a copy of each stage's output (for stagewise checks)."""
         keep = (lambda k, v: trace.__setitem__(k, v.clone())) if trace is not None else (lambda k, v: None)
         cfg, w = self.cfg, self.w
@@ -194,11 +211,11 @@ class Krea2DiT:
         B = int(x.shape[0])
         dev = x.device
         img, h, wd = patchify(x, cfg.patch)
-        img = F.linear(img, *w.first)
+        img = _linear(img, w.first)
         keep("img", img)
         t = timestep_embedding(timesteps, cfg.tdim).unsqueeze(1).to(img.dtype)
-        t = F.linear(F.gelu(F.linear(t, *w.tmlp1), approximate="tanh"), *w.tmlp2)   # [B, 1, hidden]
-        tvec = F.linear(t, *w.tproj)                                                # [B, 1, 6*hidden]
+        t = _linear(_linear(t, w.tmlp1, "gelu"), w.tmlp2)                           # [B, 1, hidden]
+        tvec = _linear(t, w.tproj)                                                  # [B, 1, 6*hidden]
         keep("t", t)
         keep("tvec", tvec)
         # text fusion on the W4A4 ops (group-1 attention)
@@ -211,11 +228,16 @@ class Krea2DiT:
             for i, tb in enumerate(w.txt):
                 ctx = text_block(cfg, tb, ctx, B, Lt, rope, zero_mod, ones_gate)
                 keep(f"txt{i}", ctx)
-        ctx = F.linear(ctx.view(B, Lt, cfg.txtdim), *w.txtmlp)
+        ctx = _linear(ctx.view(B, Lt, cfg.txtdim), w.txtmlp)
         combined = torch.cat([ctx, img], 1).contiguous()                             # [B, L, hidden]
         keep("combined", combined)
         L = int(combined.shape[1])
         freqs = rope_table(positions(Lt, h, wd, dev), cfg.axes, cfg.core.theta)
+        if image_prompt is not None:
+            if w.adapter is None:
+                raise ValueError("image_prompt needs weights with an adapter")
+            combined = w.adapter.add(combined, image_prompt, freqs=freqs, strength=strength)
+            keep("adapted", combined)
         stack = self._stack(B, L, dev)
         # DoubleSharedModulation per block: (tvec + lin_i).chunk(6), written
         # into the block loop's [6, B, hidden] modulation slots
@@ -248,11 +270,15 @@ def _norm_w(n: int, gen, device) -> torch.Tensor:
 
 
 def synthetic_dit(cfg: DiTConfig, batch: int = 1, seed: int = 0, device="cuda", keep_packed: bool = False,
-                  blocks: Optional[List[BlockWeights]] = None) -> DiTWeights:
+                  blocks: Optional[List[BlockWeights]] = None, w4_conditioning: bool = False,
+                  adapter_width: Optional[int] = None) -> DiTWeights:
     """Seeded random-init weights of the whole model (no checkpoint): the
     W4A4 projections N(0, 0.02) rotated and INT4-quantised, plain linears
     N(0, 0.02) bf16, norm multipliers ~U(0.9, 1.1), modulation vectors
-    N(0, 0.1).  ``blocks``: an existing block stack to reuse."""
+    N(0, 0.1).  ``blocks``: an existing block stack to reuse.
+    ``w4_conditioning``: the same timestep MLP, tproj and txtmlp weights as INT4
+    (those whose width is a multiple of 128); ``adapter_width``: an image-prompt
+    adapter for an encoder of that width."""
     gen = torch.Generator(device=device).manual_seed(seed + 7919)
     hid, T = cfg.core.hidden, cfg.txtdim
     txt = []
@@ -269,7 +295,7 @@ def synthetic_dit(cfg: DiTConfig, batch: int = 1, seed: int = 0, device="cuda", 
         txt.append(TextBlockWeights(norm1=_norm_w(T, gen, device), norm2=_norm_w(T, gen, device),
                                     qnorm=_norm_w(128, gen, device), knorm=_norm_w(128, gen, device),
                                     packed=packed, **prepared))
-    return DiTWeights(
+    weights = DiTWeights(
         first=_lin(hid, cfg.patch_dim, gen, device), tmlp1=_lin(hid, cfg.tdim, gen, device),
         tmlp2=_lin(hid, hid, gen, device), tproj=_lin(6 * hid, hid, gen, device), txt=txt,
         txtmlp=_lin(hid, T, gen, device),
@@ -278,3 +304,11 @@ def synthetic_dit(cfg: DiTConfig, batch: int = 1, seed: int = 0, device="cuda", 
         last_norm=_norm_w(hid, gen, device), last=_lin(cfg.patch_dim, hid, gen, device),
         blocks=blocks if blocks is not None else synthetic_blocks(cfg.core, batch, seed=seed, device=device,
                                                                   keep_packed=keep_packed))
+    if w4_conditioning:
+        for name in ("tmlp1", "tmlp2", "tproj", "txtmlp"):
+            wt, b = getattr(weights, name)
+            if wt.shape[1] % 128 == 0:
+                setattr(weights, name, W4Linear.of(wt, b))
+    if adapter_width is not None:
+        weights.adapter = synthetic_adapter(cfg.core, adapter_width, seed=seed, device=device)
+    return weights
