@@ -38,25 +38,24 @@ struct QkNormParams {
   QkNormSide side[2];
 };
 
+// The items first, first + stride, .. of one side, by one warp.  (A function of
+// the side, called with each of the two parameters: picked by index, every use
+// of a parameter became a load of its own.)
 template <typename T, int D>
-__global__ void __launch_bounds__(QKN_THREADS, 3) qk_norm_rope_kernel(const __grid_constant__ QkNormParams p) {
+__device__ __forceinline__ void qk_norm_side(const QkNormSide& s, uint32_t at, uint32_t stride) {
   constexpr int LPH = D / 8;               // lanes per head
   constexpr int HPS = 32 / LPH;            // heads per step
   constexpr int STEPS = QKN_HEADS / HPS;
   const int lane = threadIdx.x & 31;
   const int c = (lane % LPH) * 8;          // this lane's first column
-  const uint32_t total = p.side[0].items + p.side[1].items;
-  const uint32_t stride = gridDim.x * (QKN_THREADS / 32);
+  if (at >= s.items) return;
 
   struct Item {
-    int side, h0;
+    int h0;
     uint32_t b, tok;
   };
   auto locate = [&](uint32_t i) {
     Item it;
-    it.side = i >= p.side[0].items;
-    const QkNormSide& s = p.side[it.side];
-    if (it.side) i -= p.side[0].items;
     const uint32_t row = i / s.chunks;     // batch * length + token
     it.h0 = (int)(i - row * s.chunks) * QKN_HEADS + lane / LPH;
     it.b = row / s.length;
@@ -64,59 +63,47 @@ __global__ void __launch_bounds__(QKN_THREADS, 3) qk_norm_rope_kernel(const __gr
     return it;
   };
   auto load = [&](const Item& it, uint4 (&v)[STEPS]) {
-    const QkNormSide& s = p.side[it.side];
-    const T* x = static_cast<const T*>(s.x) + it.b * s.sb + it.tok * s.st + c;
+    const T* x = static_cast<const T*>(s.x) + it.b * s.sb + it.tok * s.st + it.h0 * s.sh + c;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i)
-      if (it.h0 + i * HPS < s.heads) v[i] = ldg_stream(x + (long long)(it.h0 + i * HPS) * s.sh);
+    for (int i = 0; i < STEPS; ++i) {
+      if (it.h0 + i * HPS < s.heads) v[i] = ldg_stream(x);
+      x += HPS * s.sh;
+    }
   };
+  float w[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4*>(w + i) = __ldg(reinterpret_cast<const float4*>(s.w + c + i));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] += 1.0f;
 
-  uint32_t at = blockIdx.x * (QKN_THREADS / 32) + (threadIdx.x >> 5);
-  if (at >= total) return;
   Item it = locate(at);
   uint4 v[STEPS];
   load(it, v);
   for (;;) {
     const uint32_t next = at + stride;
-    const bool more = next < total && next > at;
+    const bool more = next < s.items && next > at;
     Item nit = it;
     uint4 nv[STEPS];
     if (more) {
       nit = locate(next);
       load(nit, nv);
     }
-    const QkNormSide& s = p.side[it.side];
-    // f[4 j ..]: the pair's matrix with the norm weights of its columns, or the weights alone
-    float f[16];
-    {
-      float w[8];
-#pragma unroll
-      for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4*>(w + i) = __ldg(reinterpret_cast<const float4*>(s.w + c + i));
-      if (s.freqs) {
+    T* y = static_cast<T*>(s.y) + (((long long)it.b * s.length + it.tok) * s.heads + it.h0) * D + c;
+    auto work = [&](auto turn) {
+      float f[16];  // f[4 j ..]: the pair's matrix with the norm weights of its columns
+      if constexpr (decltype(turn)::value) {
         const float* fr = s.freqs + ((long long)(s.fb == 1 ? 0 : it.b) * s.length + it.tok) * (2 * D) + 2 * c;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const float4 m = __ldg(reinterpret_cast<const float4*>(fr + i));
-          const float w0 = w[i / 2] + 1.0f, w1 = w[i / 2 + 1] + 1.0f;
-          f[i] = m.x * w0, f[i + 1] = m.y * w1, f[i + 2] = m.z * w0, f[i + 3] = m.w * w1;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          f[i] = w[i / 2] + 1.0f, f[i + 3] = w[i / 2 + 1] + 1.0f;
-          f[i + 1] = f[i + 2] = 0.0f;
+          f[i] = m.x * w[i / 2], f[i + 1] = m.y * w[i / 2 + 1], f[i + 2] = m.z * w[i / 2], f[i + 3] = m.w * w[i / 2 + 1];
         }
       }
-    }
-    const bool turn = s.freqs != nullptr;
-    T* y = static_cast<T*>(s.y) + (((long long)it.b * s.length + it.tok) * s.heads) * D + c;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const int h = it.h0 + i * HPS;
-      const bool live = h < s.heads;
-      float e[8];
-      float sum = 0.0f;
-      if (live) {
+      for (int i = 0; i < STEPS; ++i) {
+        const bool live = it.h0 + i * HPS < s.heads;
+        float e[8];
+        float sum = 0.0f;
         const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -125,20 +112,26 @@ __global__ void __launch_bounds__(QKN_THREADS, 3) qk_norm_rope_kernel(const __gr
           e[2 * j + 1] = a.y;
           sum = fmaf(a.x, a.x, fmaf(a.y, a.y, sum));
         }
-      }
 #pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (!live) continue;
-      const float r = rsqrtf(sum * (1.0f / D) + s.eps);
-      uint32_t o[4];
+        for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float r = rsqrtf(sum * (1.0f / D) + s.eps);
+        uint32_t o[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = e[2 * j] * r, z = e[2 * j + 1] * r;
-        // (without a table the other column must not enter: 0 * inf)
-        o[j] = turn ? Elem16<T>::pack(fmaf(f[4 * j], a, f[4 * j + 1] * z), fmaf(f[4 * j + 2], a, f[4 * j + 3] * z))
-                    : Elem16<T>::pack(f[4 * j] * a, f[4 * j + 3] * z);
+        for (int j = 0; j < 4; ++j) {
+          const float a = e[2 * j] * r, z = e[2 * j + 1] * r;
+          if constexpr (decltype(turn)::value) {
+            o[j] = Elem16<T>::pack(fmaf(f[4 * j], a, f[4 * j + 1] * z), fmaf(f[4 * j + 2], a, f[4 * j + 3] * z));
+          } else {
+            o[j] = Elem16<T>::pack(w[2 * j] * a, w[2 * j + 1] * z);
+          }
+        }
+        if (live) __stcs(reinterpret_cast<uint4*>(y + i * HPS * D), make_uint4(o[0], o[1], o[2], o[3]));
       }
-      *reinterpret_cast<uint4*>(y + (long long)h * D) = make_uint4(o[0], o[1], o[2], o[3]);
+    };
+    if (s.freqs) {
+      work(std::true_type{});
+    } else {
+      work(std::false_type{});
     }
     if (!more) break;
     at = next;
@@ -146,6 +139,16 @@ __global__ void __launch_bounds__(QKN_THREADS, 3) qk_norm_rope_kernel(const __gr
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) v[i] = nv[i];
   }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(QKN_THREADS, 3) qk_norm_rope_kernel(const __grid_constant__ QkNormParams p) {
+  const uint32_t stride = gridDim.x * (QKN_THREADS / 32);
+  const uint32_t at = blockIdx.x * (QKN_THREADS / 32) + (threadIdx.x >> 5);
+  qk_norm_side<T, D>(p.side[0], at, stride);
+  // the second side goes on with the warp after the first side's last
+  const uint32_t used = p.side[0].items % stride;
+  qk_norm_side<T, D>(p.side[1], at >= used ? at - used : at + stride - used, stride);
 }
 
 }  // namespace k2b
