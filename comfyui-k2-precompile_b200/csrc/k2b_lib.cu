@@ -429,21 +429,23 @@ static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void*
   if (rc) return rc;
   p.frag = frag;
   p.factor = factor;
-  // Warps along k: one per row tile where the tiles alone give every SM its
-  // sixteen warps, else as many as it takes (a warp keeps at least two groups).
+  // Warps along k: one per row tile where the tiles alone give every SM ten
+  // warps, else as many as it takes (a warp keeps at least two groups).
   const long long row_tiles = (p.n + 15) / 16;
-  const int sel = mblocks == 1 ? 0 : mblocks == 2 ? 1 : 2;
-  const int nt = 1 << sel, gy = (mblocks + nt - 1) / nt;
+  // up to 16 rows per CTA; 32 took longer at every size (77 rows by 1536 x 2560
+  // 12.4 against 8.9 us, by 36864 x 6144 403 against 194): their operands do not
+  // fit the registers, and the loads stand in each other's way
+  const int nt = mblocks == 1 ? 1 : 2, gy = (mblocks + nt - 1) / nt;
   int sms = 0, dev = 0;
   rc = current_device(&dev);
   if (rc) return rc;
   cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return (int)e;
   p.kw = 1;
-  while (p.kw < W4_WARPS && p.groups >= 4 * p.kw && row_tiles * gy * p.kw < 15LL * sms) p.kw *= 2;
+  while (p.kw < W4_WARPS && p.groups >= 4 * p.kw && row_tiles * gy * p.kw < 10LL * sms) p.kw *= 2;
   if (gy > 65535) return (int)cudaErrorInvalidValue;
   typedef void (*Kernel)(W4Params);
-  static const Kernel kernels[3] = {w4_linear_kernel<T, 1>, w4_linear_kernel<T, 2>, w4_linear_kernel<T, 4>};
+  static const Kernel kernels[2] = {w4_linear_kernel<T, 1>, w4_linear_kernel<T, 2>};
   const int rows_per_cta = 16 * (W4_WARPS / p.kw);
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -455,7 +457,7 @@ static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void*
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, kernels[sel], p);
+  return (int)cudaLaunchKernelEx(&cfg, kernels[nt - 1], p);
 }
 
 // --------------------------------------------------------- qk_norm_rope

@@ -26,8 +26,8 @@
 // that order by the prepare kernel, one 16-byte load per word, which L1 serves
 // to the CTA's other warps.  Codes become fp16 exactly by setting the exponent
 // of 1024 around a nibble.  Each group's sum is scaled by s and the row's
-// power of two in fp32 and added up in fp32.  Three or five groups of
-// weights and scales are in flight per warp.  Where there are too few row tiles to fill
+// power of two in fp32 and added up in fp32.  Two bursts of
+// neighbouring groups are in flight per warp.  Where there are too few row tiles to fill
 // the GPU, up to eight warps share a tile along k and add up in a fixed order.
 #pragma once
 #include "elem16.cuh"
@@ -135,12 +135,15 @@ struct W4Params {
   int kw;                // warps of a CTA along k (1, 2, 4, 8); the others take further rows
 };
 
-// NT: blocks of 8 activation rows of this CTA (blockIdx.y * NT first).
+// NT: blocks of 8 activation rows of this CTA (blockIdx.y * NT first), 1 or 2.
 template <typename T, int NT>
 __global__ void __launch_bounds__(W4_THREADS, 2) w4_linear_kernel(const __grid_constant__ W4Params p) {
-  constexpr int CH = NT == 1 ? 4 : NT == 2 ? 2 : 1;
-  // groups in flight per warp: what leaves registers for two CTAs per SM
-  constexpr int DEPTH = NT == 4 ? 3 : 5;
+  // Two bursts of BURST groups per warp: a burst asks for BURST x 64
+  // neighbouring bytes of each row at once.  (Asked for group by group, five in
+  // flight, the loads alone took 27 us of 36864 x 6144 instead of 23.  Bursts
+  // of 3 and 4 cost more in registers than they give: 33 and 41 against 31 us
+  // for the whole product.)
+  constexpr int BURST = 2;
   __shared__ float red[W4_WARPS][16][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
@@ -153,21 +156,29 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_linear_kernel(const __grid_c
   const int n0 = blockIdx.x * 16 * rw;  // the CTA's first weight row
   const int ra = min(n0 + wr * 16 + r, p.n - 1), rb = min(n0 + wr * 16 + r + 8, p.n - 1);
 
-  uint4 wa[DEPTH], wb[DEPTH];
-  uint32_t sa[DEPTH], sb[DEPTH];  // fp16 scales, a register each
+  uint4 wa[2][BURST], wb[2][BURST];
+  uint32_t sa[2][BURST], sb[2][BURST];  // fp16 scales, a register each
   const uint8_t* pa = p.w + ra * row_bytes + g0 * 64 + t * 16;
   const uint8_t* pb = p.w + rb * row_bytes + g0 * 64 + t * 16;
   const unsigned short* qa = p.scales + (long long)ra * p.groups + g0;
   const unsigned short* qb = p.scales + (long long)rb * p.groups + g0;
-  auto load = [&](int s) {
-    wa[s] = ldg_stream(pa + s * 64);
-    wb[s] = ldg_stream(pb + s * 64);
-    sa[s] = ldg_ahead_u16(qa + s);
-    sb[s] = ldg_ahead_u16(qb + s);
-  };
+  // burst u of the pair that starts at the pointers, `left` groups remaining there
+  auto load = [&](int u, int left) {
 #pragma unroll
-  for (int s = 0; s < DEPTH; ++s)
-    if (s < count) load(s);
+    for (int s = 0; s < BURST; ++s)
+      if (u * BURST + s < left) {
+        wa[u][s] = ldg_stream(pa + (u * BURST + s) * 64);
+        wb[u][s] = ldg_stream(pb + (u * BURST + s) * 64);
+      }
+#pragma unroll
+    for (int s = 0; s < BURST; ++s)
+      if (u * BURST + s < left) {
+        sa[u][s] = ldg_ahead_u16(qa + u * BURST + s);
+        sb[u][s] = ldg_ahead_u16(qb + u * BURST + s);
+      }
+  };
+  load(0, count);
+  load(1, count);
   pdl_wait();
 
   // x' of row r of each block; rows past m are zero and are not read
@@ -184,21 +195,22 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_linear_kernel(const __grid_c
   float acc[NT][4];
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-  for (int i0 = 0; i0 < count; i0 += DEPTH) {
-    pa += DEPTH * 64;
-    pb += DEPTH * 64;
-    qa += DEPTH;
-    qb += DEPTH;
+  for (int i0 = 0; i0 < count; i0 += 2 * BURST) {
+    pa += 2 * BURST * 64;
+    pb += 2 * BURST * 64;
+    qa += 2 * BURST;
+    qb += 2 * BURST;
 #pragma unroll
-    for (int s = 0; s < DEPTH; ++s) {
-      if (i0 + s < count) {
-        const uint32_t ua[4] = {wa[s].x, wa[s].y, wa[s].z, wa[s].w};
-        const uint32_t ub[4] = {wb[s].x, wb[s].y, wb[s].z, wb[s].w};
-        // CH chains of products per block: one of eight would hold the warp up
-        // for 8 x 24 cycles at the scaling below
-        float c[CH][NT][4];
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int i = 0; i < CH * NT; ++i) c[i / NT][i % NT][0] = c[i / NT][i % NT][1] = c[i / NT][i % NT][2] = c[i / NT][i % NT][3] = 0.0f;
+      for (int v = 0; v < BURST; ++v) {
+        const int s = u * BURST + v;
+        if (i0 + s >= count) break;
+        const uint32_t ua[4] = {wa[u][v].x, wa[u][v].y, wa[u][v].z, wa[u][v].w};
+        const uint32_t ub[4] = {wb[u][v].x, wb[u][v].y, wb[u][v].z, wb[u][v].w};
+        float c[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t ha[4], hb[4];
@@ -208,31 +220,27 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_linear_kernel(const __grid_c
           for (int i = 0; i < NT; ++i) {
             uint4 x = make_uint4(0, 0, 0, 0);
             if (live[i]) x = *reinterpret_cast<const uint4*>(px[i] + s * W4_FRAG_BYTES + w * 512);
-            mma16816<__half>(c[w % CH][i], ha[0], hb[0], ha[1], hb[1], x.x, x.y);
-            mma16816<__half>(c[w % CH][i], ha[2], hb[2], ha[3], hb[3], x.z, x.w);
+            mma16816<__half>(c[i], ha[0], hb[0], ha[1], hb[1], x.x, x.y);
+            mma16816<__half>(c[i], ha[2], hb[2], ha[3], hb[3], x.z, x.w);
           }
         }
-        const float fa = __half2float(__ushort_as_half((unsigned short)sa[s]));
-        const float fb = __half2float(__ushort_as_half((unsigned short)sb[s]));
+        const float fa = __half2float(__ushort_as_half((unsigned short)sa[u][v]));
+        const float fb = __half2float(__ushort_as_half((unsigned short)sb[u][v]));
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           const float2 f = *reinterpret_cast<const float2*>(pf[i] + s * 8);
-#pragma unroll
-          for (int q = 1; q < CH; ++q)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[0][i][e] += c[q][i][e];
-          acc[i][0] = fmaf(c[0][i][0] * f.x, fa, acc[i][0]);
-          acc[i][1] = fmaf(c[0][i][1] * f.y, fa, acc[i][1]);
-          acc[i][2] = fmaf(c[0][i][2] * f.x, fb, acc[i][2]);
-          acc[i][3] = fmaf(c[0][i][3] * f.y, fb, acc[i][3]);
+          acc[i][0] = fmaf(c[i][0] * f.x, fa, acc[i][0]);
+          acc[i][1] = fmaf(c[i][1] * f.y, fa, acc[i][1]);
+          acc[i][2] = fmaf(c[i][2] * f.x, fb, acc[i][2]);
+          acc[i][3] = fmaf(c[i][3] * f.y, fb, acc[i][3]);
         }
-        if (i0 + s + DEPTH < count) load(s);
       }
+      load(u, count - i0 - 2 * BURST);
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      px[i] += DEPTH * W4_FRAG_BYTES;
-      pf[i] += DEPTH * 8;
+      px[i] += 2 * BURST * W4_FRAG_BYTES;
+      pf[i] += 2 * BURST * 8;
     }
   }
   // the tile's sums over its kw warps, in warp order

@@ -611,7 +611,7 @@ def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, bias:
     weight was rotated by H128 along K (model.quantize_weight), so x is too.
     act: "none", "gelu" (tanh form) or "silu".  Returns [..., N] in x's dtype,
     summed in fp32 and rounded once.  Meant for up to about a hundred rows (a
-    modulation vector, a prompt's states): every 32 rows read the weight
+    modulation vector, a prompt's states): every 16 rows read the weight
     again; above that quantise the activations and use ``gemm_bf16``."""
     _need(act in _ACT, f"w4_linear: act {act!r} is none of {', '.join(_ACT)}")
     return bind().w4_linear(x, packed, scales, bias, rotate, _ACT[act])
