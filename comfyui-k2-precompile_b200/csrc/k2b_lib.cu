@@ -418,17 +418,24 @@ template <typename T>
 static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void* work, int k, bool rotate,
                             cudaStream_t st) {
   const int mblocks = (int)w4_row_blocks(p.m);
-  uint8_t* frag = static_cast<uint8_t*>(work);
-  float* factor = reinterpret_cast<float*>(frag + (long long)mblocks * p.groups * W4_FRAG_BYTES);
-  const long long total = (long long)mblocks * 8 * p.groups;
-  if (total > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  const int pgrid = (int)((total + W4_WARPS - 1) / W4_WARPS);
-  auto prep = rotate ? w4_prepare_kernel<T, true> : w4_prepare_kernel<T, false>;
-  prep<<<pgrid, W4_THREADS, 0, st>>>(static_cast<const T*>(x), x_stride, frag, factor, p.m, p.groups, (int)total);
-  int rc = launch_status();
-  if (rc) return rc;
-  p.frag = frag;
-  p.factor = factor;
+  const bool fused = w4_fused(p.m, k);
+  int rc = 0;
+  if (fused) {
+    p.x = x;
+    p.x_stride = x_stride;
+  } else {
+    uint8_t* frag = static_cast<uint8_t*>(work);
+    float* factor = reinterpret_cast<float*>(frag + (long long)mblocks * p.groups * W4_FRAG_BYTES);
+    const long long total = (long long)mblocks * 8 * p.groups;
+    if (!work || !aligned16(work) || total > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    const int pgrid = (int)((total + W4_WARPS - 1) / W4_WARPS);
+    auto prep = rotate ? w4_prepare_kernel<T, true> : w4_prepare_kernel<T, false>;
+    prep<<<pgrid, W4_THREADS, 0, st>>>(static_cast<const T*>(x), x_stride, frag, factor, p.m, p.groups, (int)total);
+    rc = launch_status();
+    if (rc) return rc;
+    p.frag = frag;
+    p.factor = factor;
+  }
   // Warps along k: one per row tile where the tiles alone give every SM ten
   // warps, else as many as it takes (a warp keeps at least two groups).
   const long long row_tiles = (p.n + 15) / 16;
@@ -445,7 +452,8 @@ static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void*
   while (p.kw < W4_WARPS && p.groups >= 4 * p.kw && row_tiles * gy * p.kw < 10LL * sms) p.kw *= 2;
   if (gy > 65535) return (int)cudaErrorInvalidValue;
   typedef void (*Kernel)(W4Params);
-  static const Kernel kernels[2] = {w4_linear_kernel<T, 1>, w4_linear_kernel<T, 2>};
+  static const Kernel kernels[4] = {w4_linear_kernel<T, 1>, w4_linear_kernel<T, 2>, w4_linear_kernel<T, 1, true, false>,
+                                    w4_linear_kernel<T, 1, true, true>};
   const int rows_per_cta = 16 * (W4_WARPS / p.kw);
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -456,8 +464,8 @@ static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void*
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, kernels[nt - 1], p);
+  cfg.numAttrs = fused ? 0 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernels[fused ? (rotate ? 3 : 2) : nt - 1], p);
 }
 
 // --------------------------------------------------------- qk_norm_rope
@@ -948,7 +956,7 @@ K2B_EXPORT int k2b_attention_quant(const void* q, const void* k, const void* v, 
 
 // ------------------------------------------------ conditioning operators
 K2B_EXPORT long long k2b_w4_workspace_bytes(int m, int k) {
-  return m <= 0 || k <= 0 || k % 128 ? -1 : w4_workspace_bytes(m, k);
+  return m <= 0 || k <= 0 || k % 128 ? -1 : w4_fused(m, k) ? 0 : w4_workspace_bytes(m, k);
 }
 
 K2B_EXPORT int k2b_w4_linear(const void* x, long long x_stride, const void* packed, const void* scales,
@@ -957,8 +965,7 @@ K2B_EXPORT int k2b_w4_linear(const void* x, long long x_stride, const void* pack
   if (m <= 0 || n <= 0 || k <= 0 || k % 128 || x_stride < (m > 1 ? k : 0) || x_stride % 4 ||
       (dtype != COND_FP16 && dtype != COND_BF16) || act < W4_NONE || act > W4_SILU)
     return (int)cudaErrorInvalidValue;
-  if (!x || !packed || !scales || !out || !workspace || reinterpret_cast<uintptr_t>(x) % 8 || !aligned16(packed) ||
-      !aligned16(workspace))
+  if (!x || !packed || !scales || !out || reinterpret_cast<uintptr_t>(x) % 8 || !aligned16(packed))
     return (int)cudaErrorInvalidValue;
   W4Params p;
   memset(&p, 0, sizeof(p));

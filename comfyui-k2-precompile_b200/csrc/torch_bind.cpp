@@ -131,9 +131,11 @@ PyObject* w4_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     out = at::empty(shape, x.options());
     if (out.numel()) {
       const int mi = fits_int(m, "w4_linear"), ni = fits_int(n, "w4_linear"), ki = fits_int(k, "w4_linear");
-      const at::Tensor work = at::empty({(int64_t)k2b_w4_workspace_bytes(mi, ki)}, x.options().dtype(at::kByte));
+      const long long bytes = k2b_w4_workspace_bytes(mi, ki);
+      at::Tensor work;
+      if (bytes > 0) work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
       rc = k2b_w4_linear(x.data_ptr(), stride, packed.data_ptr(), scales.data_ptr(), ptr(bias), out.data_ptr(),
-                         work.data_ptr(), mi, ni, ki, code, rotate, (int)act, stream());
+                         work.defined() ? work.data_ptr() : nullptr, mi, ni, ki, code, rotate, (int)act, stream());
     }
   }
   if (rc) return failed("k2b_w4_linear", rc);

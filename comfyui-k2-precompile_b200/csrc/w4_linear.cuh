@@ -45,15 +45,21 @@ inline long long w4_workspace_bytes(int m, int k) {
   return w4_row_blocks(m) * (k / 128) * (W4_FRAG_BYTES + 8 * (long long)sizeof(float));
 }
 
-// One warp per (row, group); rows past m up to a whole block of 8 are zero.
+// Whether the product kernel prepares its rows itself, in shared memory: a few
+// rows of few groups, which a CTA does in less time than a second launch takes
+// (one row by 6144 x 256: 3.1 against 4.0 us, with the host side of the call 5.8
+// against 9.4).
+constexpr int W4_FUSED_GROUPS = 16, W4_FUSED_ITEMS = 64;
+inline bool w4_fused(int m, int k) {
+  return m <= 8 && k <= 128 * W4_FUSED_GROUPS && (long long)m * (k / 128) <= W4_FUSED_ITEMS;
+}
+
+// x' of one (row, group) by a warp, to place `at` (the group's of the row's
+// block of 8) of frag and factor; a row at or past m is zero.
 template <typename T, bool ROTATE>
-__global__ void __launch_bounds__(W4_THREADS)
-    w4_prepare_kernel(const T* x, long long x_stride, uint8_t* frag, float* factor, int m, int groups, int total) {
-  pdl_launch_dependents();
+__device__ __forceinline__ void w4_prepare(const T* x, long long x_stride, uint8_t* frag, float* factor, int m, int row,
+                                           int g, long long at) {
   const int lane = threadIdx.x & 31;
-  const int item = blockIdx.x * W4_WARPS + (threadIdx.x >> 5);
-  if (item >= total) return;
-  const int row = item / groups, g = item % groups;
   float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (row < m) {
     const uint2 u = __ldg(reinterpret_cast<const uint2*>(x + row * x_stride + g * 128 + lane * 4));
@@ -95,10 +101,20 @@ __global__ void __launch_bounds__(W4_THREADS)
     out = make_uint2(__byte_perm(lo, olo, 0x5410), __byte_perm(lo, olo, 0x7632));
   }
   const int t = lane >> 3, word = (lane >> 1) & 3;
-  const long long at = ((long long)(row >> 3) * groups + g);
   *reinterpret_cast<uint2*>(frag + at * W4_FRAG_BYTES + ((word * 8 + (row & 7)) * 4 + t) * 16 + (lane & 1) * 8) = out;
   // 1/sqrt(128) of the rotation joins the factor
   if (lane == 0) factor[at * 8 + (row & 7)] = ROTATE ? down * kHadamardScale : down;
+}
+
+// One warp per (row, group); rows past m up to a whole block of 8 are zero.
+template <typename T, bool ROTATE>
+__global__ void __launch_bounds__(W4_THREADS)
+    w4_prepare_kernel(const T* x, long long x_stride, uint8_t* frag, float* factor, int m, int groups, int total) {
+  pdl_launch_dependents();
+  const int item = blockIdx.x * W4_WARPS + (threadIdx.x >> 5);
+  if (item >= total) return;
+  const int row = item / groups, g = item % groups;
+  w4_prepare<T, ROTATE>(x, x_stride, frag, factor, m, row, g, (long long)(row >> 3) * groups + g);
 }
 
 // Eight INT4 codes (two's complement nibbles, code i in bits 4i..) -> fp16
@@ -125,9 +141,11 @@ __device__ __forceinline__ float w4_act(float y, int act) {
 }
 
 struct W4Params {
+  const void* x;         // the rows themselves (a fused launch)
+  long long x_stride;
   const uint8_t* w;      // [n, k/2]
   const unsigned short* scales;  // fp16 [n, groups]
-  const uint8_t* frag;   // prepared rows
+  const uint8_t* frag;   // prepared rows (not a fused launch)
   const float* factor;
   const void* bias;      // [n] or null
   void* out;             // [m, n]
@@ -136,7 +154,8 @@ struct W4Params {
 };
 
 // NT: blocks of 8 activation rows of this CTA (blockIdx.y * NT first), 1 or 2.
-template <typename T, int NT>
+// FUSED: the CTA prepares the rows itself, with ROTATE or without.
+template <typename T, int NT, bool FUSED = false, bool ROTATE = false>
 __global__ void __launch_bounds__(W4_THREADS, 2) w4_linear_kernel(const __grid_constant__ W4Params p) {
   // Two bursts of BURST groups per warp: a burst asks for BURST x 64
   // neighbouring bytes of each row at once.  (Asked for group by group, five in
@@ -179,7 +198,21 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_linear_kernel(const __grid_c
   };
   load(0, count);
   load(1, count);
-  pdl_wait();
+  const uint8_t* frag = p.frag;
+  const float* factor = p.factor;
+  if constexpr (FUSED) {
+    __shared__ __align__(16) uint8_t own_frag[W4_FUSED_GROUPS * W4_FRAG_BYTES];
+    __shared__ float own_factor[W4_FUSED_GROUPS * 8];
+    for (int i = warp; i < p.m * p.groups; i += W4_WARPS) {
+      const int row = i / p.groups, g = i - row * p.groups;
+      w4_prepare<T, ROTATE>(static_cast<const T*>(p.x), p.x_stride, own_frag, own_factor, p.m, row, g, g);
+    }
+    __syncthreads();
+    frag = own_frag;
+    factor = own_factor;
+  } else {
+    pdl_wait();
+  }
 
   // x' of row r of each block; rows past m are zero and are not read
   const uint8_t* px[NT];
@@ -188,8 +221,8 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_linear_kernel(const __grid_c
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     const long long at = (long long)min(block0 + i, mblocks - 1) * p.groups + g0;
-    px[i] = p.frag + at * W4_FRAG_BYTES + lane * 16;
-    pf[i] = p.factor + at * 8 + 2 * t;
+    px[i] = frag + at * W4_FRAG_BYTES + lane * 16;
+    pf[i] = factor + at * 8 + 2 * t;
     live[i] = (block0 + i) * 8 + r < p.m;
   }
   float acc[NT][4];

@@ -212,7 +212,7 @@ int k2b_attention_quant(const void* q, const void* k, const void* v, void* oq, v
  * == 0, bias [n] or null.  rotate: x' = H128/sqrt(128) of x per group of 128
  * (weights from k2b_rotate_quant), else x' = x.  act 0 none, 1 gelu (tanh
  * form), 2 silu.  workspace: k2b_w4_workspace_bytes(m, k) bytes (-1 for sizes
- * it does not take), 16-byte aligned. */
+ * it does not take), 16-byte aligned (0 bytes: may be null). */
 long long k2b_w4_workspace_bytes(int m, int k);
 int k2b_w4_linear(const void* x, long long x_stride, const void* packed, const void* scales, const void* bias,
                   void* out, void* workspace, int m, int n, int k, int dtype, int rotate, int act, void* stream);

@@ -100,11 +100,19 @@ def test_c_entries_refuse(lib):
     """cudaErrorInvalidValue for sizes, types, strides and pointers that the kernels do not take."""
     assert lib.k2b_w4_workspace_bytes(0, 128) == -1 and lib.k2b_w4_workspace_bytes(1, 100) == -1
     assert lib.k2b_w4_workspace_bytes(9, 256) >= 2 * 2 * (8 * 128 * 2)
-    w4 = lambda m=1, n=8, k=128, dtype=2, act=0, x=P, stride=128: lib.k2b_w4_linear(  # noqa: E731
-        x, stride, P, P, None, P, P, m, n, k, dtype, 1, act, None)
+    assert lib.k2b_w4_workspace_bytes(1, 256) == 0  # prepared inside the product kernel
+    # a mask that depends on the query or the head is packed for the many-query kernel: 16 bytes per row and 128 keys,
+    # and per 128 rows
+    need = lib.k2b_cross_workspace_bytes
+    assert need(1, 48, 12, 4096, 1000, 128, 0, 0, 1000) == 16 * 8 * (4096 + 32)
+    assert need(2, 48, 12, 4096, 1000, 128, 1, 1, 1) == 2 * 48 * 16 * 8 * (4096 + 32)
+    assert need(1, 48, 12, 4096, 1000, 128, 1000, 0, 0) == 0 and need(1, 48, 12, 1, 1000, 128, 0, 0, 1000) == 0
+    assert need(1, 48, 12, 4096, 0, 128, 0, 0, 1) == 0 and need(1, 47, 12, 4096, 10, 128, 0, 0, 1) == -1
+    w4 = lambda m=1, n=8, k=128, dtype=2, act=0, x=P, stride=128, work=P: lib.k2b_w4_linear(  # noqa: E731
+        x, stride, P, P, None, P, work, m, n, k, dtype, 1, act, None)
     odd = ctypes.c_void_p((1 << 20) + 2)
     assert {w4(m=0), w4(n=0), w4(k=100), w4(dtype=0), w4(act=3), w4(x=None), w4(x=odd), w4(stride=126),
-            w4(m=2, stride=64)} == {1}
+            w4(m=2, stride=64), w4(m=9, work=None), w4(k=4096, stride=4096, work=odd)} == {1}
     qk = lambda q=P, lq=1, heads=2, dim=64, st=64, fb=1, dtype=2: lib.k2b_qk_norm_rope(  # noqa: E731
         q, None, P, None, P, None, P, None, 2, lq, 0, heads, 1, dim, 64, 64, st, 0, 0, 0, fb, 1, 1e-6, 1e-6, dtype, None)
     assert {qk(q=None), qk(lq=0), qk(heads=0), qk(dim=32), qk(st=4), qk(fb=3), qk(dtype=0), qk(q=odd)} == {1}

@@ -33,6 +33,10 @@ def gen_of(cuda, seed):
     (77, 1536, 2560, FP, True, True, "none"),
     (1, 100, 16384, BF, True, False, "none"),    # the longest K of the framework's weights
     (96, 40000, 128, BF, True, False, "none"),
+    (1, 300, 2048, FP, True, True, "none"),      # the widest that one launch does
+    (4, 300, 2048, BF, True, False, "none"),
+    (5, 300, 2048, BF, True, False, "none"),     # and the first that takes two
+    (8, 129, 1024, BF, False, False, "none"),
 ])
 def test_w4_linear(cuda, m, n, k, dtype, rotate, bias, act):
     gen = gen_of(cuda, m * 1000 + n)
