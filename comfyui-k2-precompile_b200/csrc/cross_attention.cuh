@@ -62,6 +62,15 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -277,55 +286,62 @@ __global__ void __launch_bounds__(XF_THREADS, D == 64 ? xf_per_sm(64) : 0) cross
     sml[XF_ROWS + row] = sum;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < XF_ROWS * D; i += XF_THREADS) {
-    float sum = 0.0f;
+  // four columns of a row to its place, rounded once
+  auto store4 = [&](int at, float4 v, float sum) {
+    const long long rr = (long long)rt * XF_ROWS + at / D;
+    if (rr >= rows) return;
+    const long long tok = rr / p.group, head = hk * p.group + rr % p.group;
+    const float by = 1.0f / sum;
+    uint2 o = make_uint2(0u, 0u);  // a row without keys
+    if (sum != 0.0f) o = make_uint2(Elem16<T>::pack(v.x * by, v.y * by), Elem16<T>::pack(v.z * by, v.w * by));
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + ((long long)b * p.lq + tok) * p.heads * D + head * D + at % D) = o;
+  };
+  for (int at = 4 * threadIdx.x; at < XF_ROWS * D; at += 4 * XF_THREADS) {
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < XF_WARPS; ++w) sum += so[w * XF_ROWS * D + i];
-    sred[i] = sum;
-  }
-  // ---------------------------------------- join the CTAs of the cluster
-  if (p.splits > 1) {
-    cluster_sync_all();
-  } else {
-    __syncthreads();
-  }
-  const int share = XF_ROWS * D / p.splits;
-  for (int i = threadIdx.x; i < share; i += XF_THREADS) {
-    const int at = split * share + i;
-    const int row = at / D, d = at % D;
-    const long long rr = (long long)rt * XF_ROWS + row;
-    float top = -INFINITY, sum = 0.0f, val = 0.0f;
+    for (int w = 0; w < XF_WARPS; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(so + w * XF_ROWS * D + at);
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
     if (p.splits == 1) {
-      sum = sml[XF_ROWS + row];
-      val = sred[at];
+      store4(at, sum, sml[XF_ROWS + at / D]);
     } else {
-      // everything in flight before the first is used
-      float mc[XF_SPLITS], lc[XF_SPLITS], vc[XF_SPLITS];
-#pragma unroll
-      for (int c = 0; c < XF_SPLITS; ++c) {
-        mc[c] = -INFINITY, lc[c] = vc[c] = 0.0f;
-        if (c < p.splits) {
-          mc[c] = ld_cluster_f32(cluster_map(smem_u32(sml + row), c));
-          lc[c] = ld_cluster_f32(cluster_map(smem_u32(sml + XF_ROWS + row), c));
-          vc[c] = ld_cluster_f32(cluster_map(smem_u32(sred + at), c));
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < XF_SPLITS; ++c) top = fmaxf(top, mc[c]);
-#pragma unroll
-      for (int c = 0; c < XF_SPLITS; ++c) {
-        const float f = mc[c] == -INFINITY ? 0.0f : exp2_fast((mc[c] - top) * kLog2e);
-        sum = fmaf(lc[c], f, sum);
-        val = fmaf(vc[c], f, val);
-      }
-    }
-    if (rr < rows) {
-      const long long tok = rr / p.group, head = hk * p.group + rr % p.group;
-      static_cast<T*>(p.out)[((long long)b * p.lq + tok) * p.heads * D + head * D + d] =
-          Elem16<T>::from_float(sum == 0.0f ? 0.0f : val / sum);
+      *reinterpret_cast<float4*>(sred + at) = sum;
     }
   }
-  if (p.splits > 1) cluster_sync_all();  // the others may still be reading this CTA's sums
+  if (p.splits == 1) return;
+  // ---------------------------------------- join the CTAs of the cluster
+  cluster_sync_all();
+  const int share = XF_ROWS * D / p.splits;
+  for (int i = 4 * threadIdx.x; i < share; i += 4 * XF_THREADS) {
+    const int at = split * share + i, row = at / D;
+    // everything in flight before the first is used
+    float mc[XF_SPLITS], lc[XF_SPLITS];
+    float4 vc[XF_SPLITS];
+#pragma unroll
+    for (int c = 0; c < XF_SPLITS; ++c) {
+      mc[c] = -INFINITY, lc[c] = 0.0f;
+      vc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (c < p.splits) {
+        mc[c] = ld_cluster_f32(cluster_map(smem_u32(sml + row), c));
+        lc[c] = ld_cluster_f32(cluster_map(smem_u32(sml + XF_ROWS + row), c));
+        vc[c] = ld_cluster_f32x4(cluster_map(smem_u32(sred + at), c));
+      }
+    }
+    float top = -INFINITY, sum = 0.0f;
+    float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int c = 0; c < XF_SPLITS; ++c) top = fmaxf(top, mc[c]);
+#pragma unroll
+    for (int c = 0; c < XF_SPLITS; ++c) {
+      const float f = mc[c] == -INFINITY ? 0.0f : exp2_fast((mc[c] - top) * kLog2e);
+      sum = fmaf(lc[c], f, sum);
+      val.x = fmaf(vc[c].x, f, val.x), val.y = fmaf(vc[c].y, f, val.y);
+      val.z = fmaf(vc[c].z, f, val.z), val.w = fmaf(vc[c].w, f, val.w);
+    }
+    store4(at, val, sum);
+  }
+  cluster_sync_all();  // the others may still be reading this CTA's sums
 }
 
 // ------------------------------------------------------ tiles of queries
