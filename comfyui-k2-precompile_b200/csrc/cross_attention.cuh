@@ -45,6 +45,10 @@ struct CrossParams {
 // of its B operand, and 16 bytes of V that are its column of eight n8 tiles
 // (the order of d inside a product is free), and pairs the V rows of two keys
 // with byte permutes.
+//
+// Bound by latency: a warp's turn of 16 keys is one trip to memory, products
+// and a join.  Measured: 1 query of 48/12 heads by 4096 keys (25 MB) 13.1 us;
+// 16 queries of 20 heads of 64 by 729 keys, four latents, 10.0.
 constexpr int XF_THREADS = 256;
 constexpr int XF_WARPS = XF_THREADS / 32;
 constexpr int XF_ROWS = 16;
@@ -381,6 +385,13 @@ __global__ void __launch_bounds__(XF_THREADS, D == 64 ? xf_per_sm(64) : 0) cross
 //     skipped by every role.
 //   - O is rescaled in TMEM only when a row's maximum grew by more than 2^8
 //     (P and the sum then stay within fp16 and fp32; o = O / l is the same).
+//
+// Bound by the chain S -> softmax -> PV of a slot (3700 cycles for 128 keys of
+// both slots, 2050 of them products) and, for short prompts, by what an item
+// costs at its end.  Measured: 8 x 4224 queries by 2048 keys, 48/12 heads,
+// 1.78 ms, 955 TFLOP/s; 4096 queries by 1000 keys under a regional mask 105 us;
+// 2 x 4050 queries by 154 and 76 keys with addends 87 us (200 MB).  Part of the
+// exponentials as a polynomial on the FMA pipe measured slower.
 constexpr int XT_BM = 128;
 constexpr int XT_BN = 128;
 constexpr int XT_THREADS = 384;

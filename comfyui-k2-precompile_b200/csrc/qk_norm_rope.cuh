@@ -15,6 +15,9 @@
 // before it works on the present one, so that loads are always in flight.  The
 // items of a token are neighbours: its table entries come from L1 after the
 // first, and w + 1 is folded into them once per item.
+// Measured: 4050 tokens of 48 + 12 heads of 128 out of a joint projection of 72
+// (133 MB) 22.5 us, 5.9 TB/s; queries of 8 x 4224 tokens (842 MB) 132 us,
+// 6.4 TB/s.
 #pragma once
 #include "elem16.cuh"
 

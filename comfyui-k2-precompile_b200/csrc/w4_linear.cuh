@@ -26,9 +26,13 @@
 // that order by the prepare kernel, one 16-byte load per word, which L1 serves
 // to the CTA's other warps.  Codes become fp16 exactly by setting the exponent
 // of 1024 around a nibble.  Each group's sum is scaled by s and the row's
-// power of two in fp32 and added up in fp32.  Two bursts of
-// neighbouring groups are in flight per warp.  Where there are too few row tiles to fill
-// the GPU, up to eight warps share a tile along k and add up in a fixed order.
+// power of two in fp32 and added up in fp32.  Two bursts of neighbouring groups
+// are in flight per warp.  Where there are too few row tiles to fill the GPU, up
+// to eight warps share a tile along k and add up in a fixed order.
+//
+// Measured: 36864 x 6144 (117 MB) by 1 row 31.5 us, 3.7 TB/s; by 8 rows 33.1;
+// by 16 rows 43; 1536 x 2560 by 77 rows 8.1.  What is left over the loads' own
+// 23 us are dequantisation and products that 16 warps do not hide entirely.
 #pragma once
 #include "elem16.cuh"
 
