@@ -397,6 +397,11 @@ constexpr int XT_BN = 128;
 constexpr int XT_THREADS = 384;
 constexpr int XT_LAUNCH_REGS = 168;  // 65536 / 384; split 88 / 208 by setmaxnreg (128 x 88 + 256 x 208 = 384 x 168)
 constexpr float XT_RESCALE = 8.0f;   // log2 units
+// A row's reference is its maximum S * c, rounded: off by up to 2^-25 of it,
+// which P carries as a power of two.  Up to 2^24 that is half a unit; from 2^28
+// on P would leave fp16, from 2^32 on fp32.  A row with a larger maximum is done
+// again by cross_row.
+constexpr float XT_LARGEST = 16777216.0f;
 constexpr int XT_RECORDS = 8;        // steps the walk may be ahead of the slowest role
 constexpr int XT_READERS = 11;       // products (2), side data, eight softmax warps
 
@@ -650,6 +655,79 @@ __device__ __forceinline__ void tmem_st_row(uint32_t taddr, const uint32_t (&r)[
         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+// One query's row by a warp on the FMA units, scores in natural units, so that
+// the largest has an exponent of exactly 0 whatever its size (XT_LARGEST).  32
+// keys at a time: a lane's own key for the score, its own columns for PV.  Out of
+// line and once per item: a test of every tile's maximum, with S replaced by its
+// rounded product, took 87 to 90 us on 2 x 4050 queries by 154 keys and 105 to
+// 110 on 4096 by 1000 under a regional mask.
+template <typename T, int D>
+__device__ __noinline__ void cross_row(const CrossParams& p, int b, int head, int tok) {
+  constexpr int C = D / 32;
+  const int lane = threadIdx.x & 31, hk = head / p.group, n = cross_keys(p, b);
+  const T* q = static_cast<const T*>(p.q) + b * p.q_sb + head * p.q_sh + tok * p.q_st;
+  const T* k = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* v = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh + C * lane;
+  float m = -INFINITY, l = 0.0f, o[C] = {};
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    const int key = k0 + lane;
+    bool keep = key < n;
+    float s = 0.0f;
+    if (keep && p.bias) {
+      s = __ldg(p.bias + b * p.bias_sb + key);
+      keep = s != -INFINITY;
+    }
+    if (keep && p.mask) keep = __ldg(p.mask + b * p.m_sb + head * p.m_sh + tok * p.m_sq + key * p.m_sk) != 0;
+    if (keep) {
+      const uint4* qr = reinterpret_cast<const uint4*>(q);
+      const uint4* kr = reinterpret_cast<const uint4*>(k + key * p.k_st);
+      float dot = 0.0f;
+#pragma unroll 4
+      for (int i = 0; i < D / 8; ++i) {
+        const uint4 x = __ldg(qr + i), y = __ldg(kr + i);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 xf = Elem16<T>::unpack(xs[e]), yf = Elem16<T>::unpack(ys[e]);
+          dot = fmaf(xf.x, yf.x, fmaf(xf.y, yf.y, dot));
+        }
+      }
+      s = fmaf(dot, p.scale, s);
+    } else {
+      s = -INFINITY;
+    }
+    float next = s;
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, w));
+    next = fmaxf(next, m);
+    const float f = m == -INFINITY ? 0.0f : exp2_fast((m - next) * kLog2e);
+    const float e = keep ? exp2_fast((s - (next == -INFINITY ? 0.0f : next)) * kLog2e) : 0.0f;
+    m = next;
+    l = fmaf(l, f, e);
+#pragma unroll
+    for (int i = 0; i < C; ++i) o[i] *= f;
+    const uint32_t live = __ballot_sync(0xffffffffu, keep);
+#pragma unroll 4
+    for (int j = 0; j < 32; ++j) {
+      const float pj = __shfl_sync(0xffffffffu, e, j);
+      if (!((live >> j) & 1u)) continue;
+      const uint32_t* vr = reinterpret_cast<const uint32_t*>(v + (k0 + j) * p.v_st);
+#pragma unroll
+      for (int i = 0; i < C; i += 2) {
+        const float2 x = Elem16<T>::unpack(__ldg(vr + i / 2));
+        o[i] = fmaf(pj, x.x, o[i]);
+        o[i + 1] = fmaf(pj, x.y, o[i + 1]);
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+  const float by = l == 0.0f ? 0.0f : 1.0f / l;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (((long long)b * p.lq + tok) * p.heads + head) * D + C * lane);
+#pragma unroll
+  for (int i = 0; i < C; i += 2) dst[i / 2] = Elem16<T>::pack(o[i] * by, o[i + 1] * by);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(XT_THREADS, 1)
     cross_tile_kernel(const __grid_constant__ CrossMaps maps, const __grid_constant__ CrossTileParams P) {
@@ -749,6 +827,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
     const float c = p.scale * kLog2e;
     uint32_t step = 0, out_no = 0;
     float m_run = -INFINITY, l_run = 0.0f;
+    float largest = 0.0f;  // of the row's tile maxima without addends, where finite
     CrossStep st;
     for (uint32_t no = 0;
          read_step(no, st, mbar_wait_s(smem_u32(&rec_full[no % XT_RECORDS]), (no / XT_RECORDS) & 1, abort_addr, ERR_WAIT_SOFTMAX));
@@ -758,6 +837,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
       if (first) {
         m_run = -INFINITY;
         l_run = 0.0f;
+        largest = 0.0f;
       }
       if (!(st.flags & XS_EMPTY)) {
         const int s = st.load % NS;
@@ -817,6 +897,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
           m4[k] = fmax_nan(m4[k], __uint_as_float(u[k + 124]));
         }
         const float mx = cm * fmax_nan(fmax_nan(m4[0], m4[1]), fmax_nan(m4[2], m4[3]));
+        if (!adds && fabsf(mx) < INFINITY) largest = fmaxf(largest, fabsf(mx));
         // m_run is the reference of P in log2 units: -inf until the row has
         // seen a key, NaN once a score was NaN or +inf (then the row is NaN)
         float alpha = 1.0f;
@@ -901,6 +982,9 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
         }
         __syncwarp();
       }
+      uint32_t again = __ballot_sync(0xffffffffu, largest > XT_LARGEST && lane < left);
+      for (; __builtin_expect(again != 0, 0); again &= again - 1)
+        cross_row<T, D>(p, st.b, head, st.q0 + t * qstep + 32 * w4 + __ffs(again) - 1);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");

@@ -1,0 +1,74 @@
+"""The conditioning operators at the ends of their ranges."""
+import pytest
+import torch
+
+import _conditioning as R
+from k2b import ops
+from k2b._native import lib
+
+pytestmark = pytest.mark.gpu
+BF, FP = torch.bfloat16, torch.float16
+# few-row kernel; many-query kernel with an even and an odd group, D 128 and 64
+SHAPES = [(1, 8, 2, 3, 300, 128, FP), (1, 16, 4, 1000, 700, 128, FP), (1, 16, 4, 1000, 700, 128, BF),
+          (1, 5, 5, 3000, 700, 64, FP), (2, 16, 4, 1500, 700, 64, BF)]
+
+
+def gen_of(cuda, seed):
+    return torch.Generator(device=cuda).manual_seed(seed)
+
+
+def takes_tiles(B, H, Hk, Lq, Lk, D):
+    return lib().k2b_cross_workspace_bytes(B, H, Hk, Lq, Lk, D, 0, 0, 1) > 0
+
+
+def whole(cuda, B, H, L, D, dtype, seed):
+    """Heads of whole numbers -2..2: their products are exact."""
+    t = torch.randint(-2, 3, (B, L, H, D), generator=gen_of(cuda, seed), device=cuda)
+    return t.to(dtype).transpose(1, 2)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("scale", [1e6, 1e8, 1e12])
+def test_huge_scores(cuda, shape, scale):
+    """Scores whose rounding alone is more than fp16's or fp32's range of exponents: each row is the mean of the values
+    at its largest score."""
+    B, H, Hk, Lq, Lk, D, dtype = shape
+    assert takes_tiles(*shape[:6]) == (Lq > 3)
+    q, k = whole(cuda, B, H, Lq, D, dtype, 1), whole(cuda, B, Hk, Lk, D, dtype, 2)
+    v = torch.randn(B, Hk, Lk, D, generator=gen_of(cuda, 3), device=cuda).to(dtype)
+    for kk in (k, -k.abs()):  # the second: scores below zero for queries above
+        qq = q if kk is k else q.abs() + 1
+        s = qq.double() @ kk.double().repeat_interleave(H // Hk, 1).transpose(-1, -2)
+        p = (s == s.amax(-1, keepdim=True)).double()
+        p /= p.sum(-1, keepdim=True)
+        vv = v.double().repeat_interleave(H // Hk, 1)
+        want = (p @ vv).transpose(1, 2).reshape(B, Lq, H * D)
+        # weights of 1 as stored; the sum and its reciprocal round in fp32, the output once
+        bound = R.UNIT[dtype] * want.abs() + 2.0 ** -20 * float(v.abs().max())
+        R.check(ops.cross_attention(qq, kk, v, scale=scale), want, bound)
+
+
+@pytest.mark.parametrize("shape", SHAPES[1:])
+def test_huge_scores_of_some_keys(cuda, shape):
+    """The same where lengths, a mask per query and addends (to the keys past the first tile) take part."""
+    B, H, Hk, Lq, Lk, D, dtype = shape
+    assert takes_tiles(*shape[:6])
+    gen = gen_of(cuda, 9)
+    q, k = whole(cuda, B, H, Lq, D, dtype, 1), whole(cuda, B, Hk, Lk, D, dtype, 2)
+    v = torch.randn(B, Hk, Lk, D, generator=gen, device=cuda).to(dtype)
+    lengths = torch.full((B,), Lk - 50, dtype=torch.int32, device=cuda)
+    mask = torch.rand(1, 1, Lq, Lk, generator=gen, device=cuda) < 0.3
+    mask[:, :, ::7] = False
+    bias = torch.randint(0, 2, (1, Lk), generator=gen, device=cuda) * 5e7
+    bias[:, :128] = 0.0
+    gone = ~R.keep_mask(B, 1, 1, Lk, lengths, None, None, cuda)[0, 0, 0]
+    v[:, :, gone] = float("nan")
+    keep = R.keep_mask(B, H, Lq, Lk, lengths, mask, None, cuda)
+    s = q.double() @ k.double().repeat_interleave(H // Hk, 1).transpose(-1, -2) * 1e8 + bias.double()
+    s = torch.where(keep, s, -torch.inf)
+    p = ((s == s.amax(-1, keepdim=True)) & keep).double()
+    p /= p.sum(-1, keepdim=True).clamp(min=1)
+    vv = torch.where(gone[:, None], 0.0, v.double()).repeat_interleave(H // Hk, 1)
+    want = (p @ vv).transpose(1, 2).reshape(B, Lq, H * D)
+    got = ops.cross_attention(q, k, v, scale=1e8, lengths=lengths, mask=mask, bias=bias)
+    R.check(got, want, R.UNIT[dtype] * want.abs() + 2.0 ** -20 * float(vv.abs().max()))
