@@ -516,6 +516,16 @@ __device__ __forceinline__ uint4 cross_seen(const CrossTileParams& P, int b, int
   return r;
 }
 
+// An addend in log2 units.  Past 2^127 those leave fp32: the rest of the range is
+// laid out evenly over what fp32 has left, so that a finite addend stays finite
+// and the larger of two stays the larger (one ulp there is 2^104: which of two
+// keys gets all of the weight is all that an addend of this size says).
+__device__ __forceinline__ float cross_addend(float raw) {
+  constexpr float kPower = 1.7014118346046923e38f;  // 2^127
+  const float over = fabsf(raw) - kPower;
+  return over > 0.0f && over < INFINITY ? copysignf(fmaf(over, 0.55f, kPower * kLog2e), raw) : raw * kLog2e;
+}
+
 __device__ __forceinline__ int cross_keys(const CrossParams& p, int b) {
   return p.lengths ? min(max(__ldg(p.lengths + b), 0), p.lk) : p.lk;
 }
@@ -1187,10 +1197,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
           if (keep && p.bias) {
             const float raw = __ldg(p.bias + st.b * p.bias_sb + key);
             keep = raw != -INFINITY;
-            // log2 units; a finite addend stays finite
-            add[c] = raw * kLog2e;
-            if (fabsf(raw) <= 3.4028234663852886e38f) add[c] = fminf(fmaxf(add[c], -3.4028234663852886e38f), 3.4028234663852886e38f);
-            if (!keep) add[c] = 0.0f;
+            add[c] = keep ? cross_addend(raw) : 0.0f;
           }
           if (keep && key_mask) keep = __ldg(p.mask + st.b * p.m_sb + key * p.m_sk) != 0;
           word[c] = __ballot_sync(0xffffffffu, keep);

@@ -72,3 +72,18 @@ def test_huge_scores_of_some_keys(cuda, shape):
     want = (p @ vv).transpose(1, 2).reshape(B, Lq, H * D)
     got = ops.cross_attention(q, k, v, scale=1e8, lengths=lengths, mask=mask, bias=bias)
     R.check(got, want, R.UNIT[dtype] * want.abs() + 2.0 ** -20 * float(vv.abs().max()))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("low,high", [(torch.finfo(torch.float32).min, -2.5e38), (2.5e38, torch.finfo(torch.float32).max),
+                                      (torch.finfo(torch.float32).min, -2.9e38)])
+@pytest.mark.parametrize("key", [3, 200])
+def test_bias_of_extreme_size(cuda, shape, low, high, key):
+    """Addends that log2 units cannot hold keep their order: the key with the larger one takes all of the weight."""
+    B, H, Hk, Lq, Lk, D, dtype = shape
+    q, k = whole(cuda, B, H, Lq, D, dtype, 1), whole(cuda, B, Hk, Lk, D, dtype, 2)
+    v = torch.randn(B, Hk, Lk, D, generator=gen_of(cuda, 3), device=cuda).to(dtype)
+    bias = torch.full((1, Lk), low, device=cuda)
+    bias[0, key] = high
+    got = ops.cross_attention(q, k, v, bias=bias).view(B, Lq, H, D)
+    assert torch.equal(got, v[:, :, key].repeat_interleave(H // Hk, 1)[:, None].expand(B, Lq, H, D))
