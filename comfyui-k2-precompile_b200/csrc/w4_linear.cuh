@@ -70,7 +70,15 @@ __device__ __forceinline__ void w4_prepare(const T* x, long long x_stride, uint8
     const float2 a = Elem16<T>::unpack(u.x), b = Elem16<T>::unpack(u.y);
     v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
   }
+  float scale = ROTATE ? kHadamardScale : 1.0f;  // what v still has to be multiplied by
   if (ROTATE) {
+    // 128 terms of more than 2^120 could leave fp32 before they are scaled
+    const float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    if (__any_sync(0xffffffffu, most > 1.329227995784916e36f)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] *= 0.00390625f;
+      scale *= 256.0f;
+    }
     const float a = v[0] + v[1], b = v[0] - v[1], c = v[2] + v[3], d = v[2] - v[3];
     v[0] = a + c, v[1] = b + d, v[2] = a - c, v[3] = b - d;
 #pragma unroll
@@ -107,7 +115,7 @@ __device__ __forceinline__ void w4_prepare(const T* x, long long x_stride, uint8
   const int t = lane >> 3, word = (lane >> 1) & 3;
   *reinterpret_cast<uint2*>(frag + at * W4_FRAG_BYTES + ((word * 8 + (row & 7)) * 4 + t) * 16 + (lane & 1) * 8) = out;
   // 1/sqrt(128) of the rotation joins the factor
-  if (lane == 0) factor[at * 8 + (row & 7)] = ROTATE ? down * kHadamardScale : down;
+  if (lane == 0) factor[at * 8 + (row & 7)] = down * scale;
 }
 
 // One warp per (row, group); rows past m up to a whole block of 8 are zero.
@@ -266,10 +274,11 @@ __global__ void __launch_bounds__(W4_THREADS, 2) w4_linear_kernel(const __grid_c
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           const float2 f = *reinterpret_cast<const float2*>(pf[i] + s * 8);
-          acc[i][0] = fmaf(c[i][0] * f.x, fa, acc[i][0]);
-          acc[i][1] = fmaf(c[i][1] * f.y, fa, acc[i][1]);
-          acc[i][2] = fmaf(c[i][2] * f.x, fb, acc[i][2]);
-          acc[i][3] = fmaf(c[i][3] * f.y, fb, acc[i][3]);
+          // (the weight's scale first: the row's alone can take a sum out of fp32)
+          acc[i][0] = fmaf(c[i][0] * fa, f.x, acc[i][0]);
+          acc[i][1] = fmaf(c[i][1] * fa, f.y, acc[i][1]);
+          acc[i][2] = fmaf(c[i][2] * fb, f.x, acc[i][2]);
+          acc[i][3] = fmaf(c[i][3] * fb, f.y, acc[i][3]);
         }
       }
       load(u, count - i0 - 2 * BURST);

@@ -87,3 +87,17 @@ def test_bias_of_extreme_size(cuda, shape, low, high, key):
     bias[0, key] = high
     got = ops.cross_attention(q, k, v, bias=bias).view(B, Lq, H, D)
     assert torch.equal(got, v[:, :, key].repeat_interleave(H // Hk, 1)[:, None].expand(B, Lq, H, D))
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 64, 512), (8, 300, 1024), (20, 64, 640)])
+@pytest.mark.parametrize("rotate", [False, True])
+def test_w4_linear_large_activations(cuda, m, n, k, rotate):
+    """Activations near the end of bf16's range, whose sums before the scales leave it: the products do not."""
+    gen = gen_of(cuda, m)
+    packed, scales = R.random_w4(n, k, gen, cuda)
+    x = torch.randn(m, k, generator=gen, device=cuda) * 1e37
+    x[-1] = 2e37  # every group's rotation adds up to 128 of these before it is scaled
+    x = x.to(BF)
+    want, bound = R.w4_linear(x, packed, scales, None, rotate, "none")
+    assert float(want.abs().max()) < 3e38
+    R.check(ops.w4_linear(x, packed, scales, rotate=rotate), want, bound)
