@@ -450,14 +450,12 @@ static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void*
   if (e != cudaSuccess) return (int)e;
   p.kw = 1;
   while (p.kw < W4_WARPS && p.groups >= 4 * p.kw && row_tiles * gy * p.kw < 10LL * sms) p.kw *= 2;
-  if (gy > 65535) return (int)cudaErrorInvalidValue;
   typedef void (*Kernel)(W4Params);
   static const Kernel kernels[4] = {w4_linear_kernel<T, 1>, w4_linear_kernel<T, 2>, w4_linear_kernel<T, 1, true, false>,
                                     w4_linear_kernel<T, 1, true, true>};
   const int rows_per_cta = 16 * (W4_WARPS / p.kw);
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((p.n + rows_per_cta - 1) / rows_per_cta, gy, 1);
   cfg.blockDim = dim3(W4_THREADS, 1, 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -465,7 +463,18 @@ static int w4_linear_launch(const void* x, long long x_stride, W4Params p, void*
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = fused ? 0 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, kernels[fused ? (rotate ? 3 : 2) : nt - 1], p);
+  constexpr int kGridY = 65535;  // a million rows; more take further launches
+  for (int y = 0; y < gy; y += kGridY) {
+    cfg.gridDim = dim3((p.n + rows_per_cta - 1) / rows_per_cta, gy - y < kGridY ? gy - y : kGridY, 1);
+    rc = (int)cudaLaunchKernelEx(&cfg, kernels[fused ? (rotate ? 3 : 2) : nt - 1], p);
+    if (rc || gy - y <= kGridY) break;
+    const long long blocks = (long long)kGridY * nt;  // of 8 rows
+    p.frag += blocks * p.groups * W4_FRAG_BYTES;
+    p.factor += blocks * p.groups * 8;
+    p.out = static_cast<T*>(p.out) + blocks * 8 * p.n;
+    p.m -= (int)blocks * 8;
+  }
+  return rc;
 }
 
 // --------------------------------------------------------- qk_norm_rope

@@ -101,3 +101,14 @@ def test_w4_linear_large_activations(cuda, m, n, k, rotate):
     want, bound = R.w4_linear(x, packed, scales, None, rotate, "none")
     assert float(want.abs().max()) < 3e38
     R.check(ops.w4_linear(x, packed, scales, rotate=rotate), want, bound)
+
+
+def test_w4_linear_rows_past_a_grid_dimension(cuda):
+    """More than 65535 blocks of 16 rows."""
+    gen = gen_of(cuda, 5)
+    m, n, k = 16 * 65535 + 21, 8, 128
+    packed, scales = R.random_w4(n, k, gen, cuda)
+    x = torch.randn(m, k, generator=gen, device=cuda).to(BF)
+    got = ops.w4_linear(x, packed, scales)
+    for rows in (slice(0, 40), slice(16 * 65535 - 20, m)):
+        R.check(got[rows], *R.w4_linear(x[rows], packed, scales, None, True, "none"))
