@@ -440,13 +440,15 @@ struct CrossTileParams {
 // Packs a mask that depends on the query or the head: one CTA per 128 rows
 // and 128 keys.
 __global__ void __launch_bounds__(256)
-    cross_mask_kernel(const uint8_t* mask, long long m_sb, long long m_sh, long long m_sq, long long m_sk, int mh,
-                      int mq, int lk, int nkt, uint4* bits, uint4* cols) {
+    cross_mask_kernel(const uint8_t* mask, long long m_sb, long long m_sh, long long m_sq, long long m_sk, int planes,
+                      int mh, int mq, int lk, int nkt, uint4* bits, uint4* cols) {
   pdl_launch_dependents();
   __shared__ uint32_t any[8][4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kt = blockIdx.x % nkt, qt = blockIdx.x / nkt;
-  const int b = blockIdx.y / mh, h = blockIdx.y % mh;
+  const int plane = blockIdx.z * gridDim.y + blockIdx.y;  // of 65535 and more
+  if (plane >= planes) return;
+  const int b = plane / mh, h = plane % mh;
   uint32_t seen[4] = {0, 0, 0, 0};
   const uint8_t* base = mask + b * m_sb + h * m_sh;
   const int key0 = kt * 128 + lane;
@@ -471,7 +473,7 @@ __global__ void __launch_bounds__(256)
         seen[c] |= w[c];
       }
       if (lane == 0 && row < mq)
-        bits[((long long)blockIdx.y * mq + row) * nkt + kt] = make_uint4(w[0], w[1], w[2], w[3]);
+        bits[((long long)plane * mq + row) * nkt + kt] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
   if (lane < 4) any[warp][lane] = lane == 0 ? seen[0] : lane == 1 ? seen[1] : lane == 2 ? seen[2] : seen[3];
@@ -480,7 +482,7 @@ __global__ void __launch_bounds__(256)
     uint32_t a[4] = {0, 0, 0, 0};
     for (int w = 0; w < 8; ++w)
       for (int c = 0; c < 4; ++c) a[c] |= any[w][c];
-    cols[((long long)blockIdx.y * ((mq + 127) / 128) + qt) * nkt + kt] = make_uint4(a[0], a[1], a[2], a[3]);
+    cols[((long long)plane * ((mq + 127) / 128) + qt) * nkt + kt] = make_uint4(a[0], a[1], a[2], a[3]);
   }
 }
 

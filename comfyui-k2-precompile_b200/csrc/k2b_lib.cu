@@ -620,15 +620,16 @@ static int cross_tile_launch(const CrossParams& p, void* work, int dim, int dtyp
   const long long items = (long long)P.pairs * P.qtiles * p.kvheads * p.batch;
   if (items > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   if (e.bytes) {
-    const long long gx = (long long)e.nkt * ((e.mq + 127) / 128), gy = (long long)e.mb * e.mh;
-    if (!work || !aligned16(work) || gx > 0x7fffffffLL || gy > 65535) return (int)cudaErrorInvalidValue;
+    const long long gx = (long long)e.nkt * ((e.mq + 127) / 128), planes = (long long)e.mb * e.mh;
+    const unsigned gy = planes < 65535 ? (unsigned)planes : 65535u;
+    if (!work || !aligned16(work) || gx > 0x7fffffffLL || planes > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     P.mb = e.mb, P.mh = e.mh, P.mq = e.mq;
     uint4* bits = static_cast<uint4*>(work);
     uint4* cols = reinterpret_cast<uint4*>(static_cast<uint8_t*>(work) + e.bits_bytes);
     P.bits = bits;
     P.cols = cols;
-    cross_mask_kernel<<<dim3((unsigned)gx, (unsigned)gy), 256, 0, st>>>(p.mask, p.m_sb, p.m_sh, p.m_sq, p.m_sk, e.mh,
-                                                                      e.mq, p.lk, e.nkt, bits, cols);
+    cross_mask_kernel<<<dim3((unsigned)gx, gy, (unsigned)((planes + gy - 1) / gy)), 256, 0, st>>>(
+        p.mask, p.m_sb, p.m_sh, p.m_sq, p.m_sk, (int)planes, e.mh, e.mq, p.lk, e.nkt, bits, cols);
     rc = launch_status();
     if (rc) return rc;
   }

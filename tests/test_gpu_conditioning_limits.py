@@ -112,3 +112,20 @@ def test_w4_linear_rows_past_a_grid_dimension(cuda):
     got = ops.w4_linear(x, packed, scales)
     for rows in (slice(0, 40), slice(16 * 65535 - 20, m)):
         R.check(got[rows], *R.w4_linear(x[rows], packed, scales, None, True, "none"))
+
+
+@pytest.mark.parametrize("per_head", [True, False])
+def test_masks_past_a_grid_dimension(cuda, per_head):
+    """A mask of its own for each of more than 65535 heads (or latents) on the many-query kernel."""
+    H, Hk, Lq, Lk, D = 4, 2, 130, 40, 64
+    B = 16400 if per_head else 65600
+    assert takes_tiles(B, H, Hk, Lq, Lk, D)
+    gen = gen_of(cuda, 6)
+    q = torch.randn(B if per_head else 1, Lq, H, D, generator=gen, device=cuda).to(BF).transpose(1, 2)
+    if not per_head:
+        q = q.repeat(B, 1, 1, 1)
+    k = torch.randn(1, Lk, Hk, D, generator=gen, device=cuda).to(BF).transpose(1, 2)
+    mask = torch.rand((B, H, 1, Lk) if per_head else (B, 1, Lq, Lk), generator=gen, device=cuda) < 0.5
+    got = ops.cross_attention(q, k, k, mask=mask)
+    for i in (slice(0, 2), slice(B // 2, B // 2 + 2), slice(B - 2, B)):
+        R.check(got[i], *R.cross_attention(q[i], k, k, None, mask[i]))
