@@ -1044,8 +1044,8 @@ K2B_EXPORT int k2b_cross_attention(const void* q, const void* k, const void* v, 
       (lengths && reinterpret_cast<uintptr_t>(lengths) % 4) || (bias && reinterpret_cast<uintptr_t>(bias) % 4))
     return (int)cudaErrorInvalidValue;
   const long long strides[9] = {q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st};
-  for (long long s : strides)
-    if (s < 0 || s % 8) return (int)cudaErrorInvalidValue;
+  for (int i = 0; i < (lk > 0 ? 9 : 3); ++i)  // without keys K and V are not read
+    if (strides[i] < 0 || strides[i] % 8) return (int)cudaErrorInvalidValue;
   CrossParams p;
   memset(&p, 0, sizeof(p));
   p.q = q, p.k = k, p.v = v, p.out = out;

@@ -129,3 +129,11 @@ def test_masks_past_a_grid_dimension(cuda, per_head):
     got = ops.cross_attention(q, k, k, mask=mask)
     for i in (slice(0, 2), slice(B // 2, B // 2 + 2), slice(B - 2, B)):
         R.check(got[i], *R.cross_attention(q[i], k, k, None, mask[i]))
+
+
+def test_cross_attention_no_keys_of_any_stride(cuda):
+    """K and V without a key: nothing is read, so their strides do not matter."""
+    q = torch.randn(2, 4, 5, 64, device=cuda).to(BF)
+    k = torch.zeros(2, 9, 260, device=cuda, dtype=BF)[:, :, :256].unflatten(2, (4, 64)).transpose(1, 2)[:, :, :0]
+    assert k.stride(2) % 8
+    assert not ops.cross_attention(q, k, k).any()
