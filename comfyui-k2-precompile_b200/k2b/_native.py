@@ -11,7 +11,6 @@ import os
 import threading
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libk2b.so")
-BIND_PATH = os.path.join(os.path.dirname(LIB_PATH), "_bind.so")
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -103,17 +102,30 @@ class K2BError(RuntimeError):
     """A libk2b entry point returned a non-zero status."""
 
 
-def _build() -> None:
-    """Build both libraries if this is a source tree without them."""
+def bind_path() -> str:
+    """The native binding's file for this Python and torch: it depends on the C++
+    ABI of both, so its name holds them, and another environment's is never
+    loaded."""
+    import sysconfig
+
+    import torch
+
+    tag = f"{sysconfig.get_config_var('SOABI')}-torch{torch.__version__}-cxx{int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+    return os.path.join(os.path.dirname(LIB_PATH), f"_bind.{tag}.so")
+
+
+def _build(what: str, path: str) -> None:
+    """Build one of the two libraries (build.py's function ``what``) if this is a
+    source tree."""
     build_py = os.path.join(os.path.dirname(os.path.dirname(LIB_PATH)), "..", "build.py")
     if not os.path.exists(build_py):
-        raise K2BError(f"libk2b not built: {LIB_PATH} is missing")
+        raise K2BError(f"libk2b not built: {path} is missing")
     import importlib.util
 
     spec = importlib.util.spec_from_file_location("_k2b_build", build_py)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
-    mod.build()
+    getattr(mod, what)()
 
 
 def lib() -> ctypes.CDLL:
@@ -122,7 +134,7 @@ def lib() -> ctypes.CDLL:
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):
-                _build()
+                _build("build_lib", LIB_PATH)
             L = ctypes.CDLL(LIB_PATH)
             for name, (res, args) in SIGNATURES.items():
                 fn = getattr(L, name)
@@ -140,12 +152,13 @@ def bind():
         lib()
         with _lock:
             if _bind is None:
-                if not os.path.exists(BIND_PATH):
-                    _build()
+                path = bind_path()
+                if not os.path.exists(path):
+                    _build("build_bind", path)
                 import importlib.machinery
                 import importlib.util
 
-                loader = importlib.machinery.ExtensionFileLoader("_bind", BIND_PATH)
+                loader = importlib.machinery.ExtensionFileLoader("_bind", path)
                 mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_bind", loader))
                 loader.exec_module(mod)
                 _bind = mod
