@@ -58,7 +58,11 @@ class W4Linear:
         return cls(packed, scales, bias, rotate)
 
     def __call__(self, x: torch.Tensor, act: str = "none") -> torch.Tensor:
-        return ops.w4_linear(x, self.packed, self.scales, self.bias, rotate=self.rotate, act=act)
+        """x [..., k]; rows that are not evenly spaced (a slice of a batch of
+        sequences) are copied together."""
+        rows = x if x.is_contiguous() else x.reshape(-1, x.shape[-1])
+        y = ops.w4_linear(rows, self.packed, self.scales, self.bias, rotate=self.rotate, act=act)
+        return y.view(*x.shape[:-1], y.shape[-1])
 
 
 @dataclass
