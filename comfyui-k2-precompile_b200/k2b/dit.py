@@ -252,7 +252,7 @@ class Krea2DiT:
         y = ops.norm_mod(stream, w.last_norm, scale.reshape(B, hidden).contiguous(),
                          shift.reshape(B, hidden).contiguous(), length=L, eps=cfg.core.eps)
         keep("normed", y)
-        out = F.linear(y.view(B, L, hidden)[:, Lt:], *w.last)
+        out = _linear(y.view(B, L, hidden)[:, Lt:], w.last)
         return unpatchify(out, h, wd, cfg.patch, cfg.channels)
 
 

@@ -36,3 +36,37 @@ def test_adapter_keys_of_a_slice(cuda):
     states = torch.randn(2, 33, 640, generator=torch.Generator(device=cuda).manual_seed(2), device=cuda).to(BF)
     got, want = a.keys(states[:, 1:]), a.keys(states[:, 1:].contiguous())
     assert torch.equal(got.k, want.k) and torch.equal(got.v, want.v)
+
+
+def small_dit(cuda, **options):
+    from k2b.dit import DiTConfig, synthetic_dit
+    from k2b.model import ModelConfig
+
+    core = ModelConfig(hidden=512, heads=4, kvheads=2, mlp=1024, blocks=1)
+    cfg = DiTConfig(core=core, channels=4, patch=2, tdim=256, txtdim=512, txt_heads=4, txt_kvheads=4, txt_mlp=1024,
+                    txt_layers=1)
+    return cfg, synthetic_dit(cfg, batch=2, seed=5, device=cuda, **options)
+
+
+def forward(cuda, cfg, weights, tokens, trace=None):
+    from k2b.dit import Krea2DiT
+
+    gen = torch.Generator(device=cuda).manual_seed(4)
+    x = torch.randn(2, 4, 16, 12, generator=gen, device=cuda).to(BF)
+    ctx = torch.randn(2, tokens, 512, generator=gen, device=cuda).to(BF)
+    return Krea2DiT(cfg, weights).forward(x, torch.tensor([0.3, 0.9], device=cuda), ctx, trace=trace)
+
+
+def test_last_linear(cuda):
+    """The projection behind the blocks, whose rows are a slice of the stream, as INT4."""
+    from k2b.adapter import W4Linear
+    from k2b.dit import unpatchify
+
+    cfg, w = small_dit(cuda)
+    w.last = W4Linear.of(*w.last)
+    trace = {}
+    got = forward(cuda, cfg, w, 7, trace)
+    rows = trace["normed"].view(2, -1, 512)[:, 7:].contiguous()
+    want, bound = R.w4_linear(rows, w.last.packed, w.last.scales, w.last.bias, w.last.rotate, "none")
+    h, wd = 8, 6
+    R.check(got, unpatchify(want, h, wd, cfg.patch, cfg.channels), unpatchify(bound, h, wd, cfg.patch, cfg.channels))
