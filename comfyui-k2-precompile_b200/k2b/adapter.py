@@ -48,14 +48,31 @@ class W4Linear:
     scales: torch.Tensor            # fp16 [n, k/128]
     bias: Optional[torch.Tensor] = None
     rotate: bool = True             # the weight was rotated along k (quantize_weight)
+    dense: Optional[torch.Tensor] = None  # bf16 [n, k]: the same weight for calls of many rows (k2b.dit)
 
     @classmethod
-    def of(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "W4Linear":
+    def of(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, dense: bool = False) -> "W4Linear":
         """Quantises a plain linear's weight [n, k]; rotated where the library's
-        quantiser takes the width (k a multiple of 512)."""
+        quantiser takes the width (k a multiple of 512).  ``dense``: keeps what
+        the codes stand for in bf16 as well."""
         rotate = weight.shape[1] % 512 == 0
         packed, scales = quantize_weight(weight) if rotate else pack_w4(weight)
-        return cls(packed, scales, bias, rotate)
+        made = cls(packed, scales, bias, rotate)
+        if dense:
+            made.dense = made.expand()
+        return made
+
+    def expand(self) -> torch.Tensor:
+        """The weight that the codes and scales stand for, unrotated, bf16 [n, k]."""
+        n, k = self.packed.shape[0], 2 * self.packed.shape[1]
+        codes = torch.stack([self.packed & 15, self.packed >> 4], -1).view(n, k // 128, 128).float()
+        w = torch.where(codes > 7, codes - 16, codes) * self.scales.float()[..., None]
+        if self.rotate:
+            h = torch.ones(1, 1, device=w.device)
+            while h.shape[0] < 128:
+                h = torch.cat([torch.cat([h, h], 1), torch.cat([h, -h], 1)])
+            w = w @ (h * 128 ** -0.5)
+        return w.view(n, k).to(torch.bfloat16)
 
     def __call__(self, x: torch.Tensor, act: str = "none") -> torch.Tensor:
         """x [..., k]; rows that are not evenly spaced (a slice of a batch of

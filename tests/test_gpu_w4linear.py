@@ -70,3 +70,40 @@ def test_last_linear(cuda):
     want, bound = R.w4_linear(rows, w.last.packed, w.last.scales, w.last.bias, w.last.rotate, "none")
     h, wd = 8, 6
     R.check(got, unpatchify(want, h, wd, cfg.patch, cfg.channels), unpatchify(bound, h, wd, cfg.patch, cfg.channels))
+
+
+@pytest.mark.parametrize("tokens", [8, 9, 60])
+def test_prompts_of_many_rows(cuda, monkeypatch, tokens):
+    """The few-row product is not asked for more rows than it reads its weight once for, and the plain linear that
+    takes them has the same weight."""
+    import torch.nn.functional as F
+
+    from k2b import ops
+
+    cfg, w = small_dit(cuda, w4_conditioning=True)
+    rows, few = [], ops.w4_linear
+    monkeypatch.setattr(ops, "w4_linear", lambda x, *a, **k: (rows.append(x.numel() // x.shape[-1]), few(x, *a, **k))[1])
+    trace = {}
+    forward(cuda, cfg, w, tokens, trace)
+    assert max(rows) <= 16 and (2 * tokens in rows) == (2 * tokens <= 16)
+    ctx, got = trace["txt0"].view(2, tokens, 512), trace["combined"][:, :tokens]
+    if 2 * tokens > 16:
+        assert torch.equal(got, F.linear(ctx, w.txtmlp.dense, w.txtmlp.bias))
+    want, bound = R.w4_linear(ctx, w.txtmlp.packed, w.txtmlp.scales, w.txtmlp.bias, w.txtmlp.rotate, "none")
+    # and the dense form rounds each weight to bf16, relative to itself
+    mag = ctx.double().abs() @ w.txtmlp.dense.double().abs().t()
+    R.check(got, want, bound + 2.0 ** -7 * mag)
+
+
+@pytest.mark.parametrize("k", [512, 640])
+def test_expanded_weight(cuda, k):
+    """The bf16 form is the packed one, rounded once: 128 fp32 terms of a row of H / sqrt(128) before it."""
+    w, _ = linear_of(cuda, 96, k, 3)
+    want = R.codes_of(w.packed).double().view(96, k // 128, 128) * w.scales.double()[..., None]
+    mag = want.abs()
+    if w.rotate:
+        h = R.hadamard(cuda)
+        want, mag = want @ h, mag @ h.abs()
+    want, mag = want.reshape(96, k), mag.reshape(96, k)
+    # (compared, not divided: a code of zero has a bound of zero)
+    assert ((w.expand().double() - want).abs() <= R.UNIT[BF] * want.abs() + 2.0 ** -16 * mag).all()
