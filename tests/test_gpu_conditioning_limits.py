@@ -137,3 +137,46 @@ def test_cross_attention_no_keys_of_any_stride(cuda):
     k = torch.zeros(2, 9, 260, device=cuda, dtype=BF)[:, :, :256].unflatten(2, (4, 64)).transpose(1, 2)[:, :, :0]
     assert k.stride(2) % 8
     assert not ops.cross_attention(q, k, k).any()
+
+
+@pytest.mark.parametrize("Lq", [1, 300])
+def test_cross_attention_offsets_past_32_bits(cuda, Lq):
+    """Keys whose elements lie beyond 2^31, on both kernels: a few at either end are left, the others excluded."""
+    H, Hk, Lk, D = 16, 2, 8_500_001, 128
+    assert takes_tiles(1, H, Hk, Lq, Lk, D) == (Lq > 1)
+    gen = gen_of(cuda, 12)
+    q = torch.randn(1, Lq, H, D, generator=gen, device=cuda).to(BF).transpose(1, 2)
+    k, v = (torch.randn(1, Lk, Hk, D, generator=gen, device=cuda, dtype=BF).transpose(1, 2) for _ in range(2))
+    assert k.stride(2) * (Lk - 1) > 2 ** 31
+    left = torch.cat([torch.arange(7), torch.arange(Lk - 90, Lk - 1)]).to(cuda)
+    bias = torch.full((1, Lk), -torch.inf, device=cuda)
+    bias[0, left] = 0.5
+    mask = torch.zeros(1, 1, 1, Lk, dtype=torch.bool, device=cuda)
+    mask[..., left] = True
+    lengths = torch.tensor([Lk - 1], dtype=torch.int32, device=cuda)
+    want, bound = R.cross_attention(q, k[:, :, left], v[:, :, left])
+    R.check(ops.cross_attention(q, k, v, bias=bias, lengths=lengths), want, bound + 2.0 ** -16 * float(v[:, :, left].abs().max()))
+    R.check(ops.cross_attention(q, k, v, mask=mask), want, bound)
+
+
+def test_qk_norm_rope_offsets_past_32_bits(cuda):
+    gen = gen_of(cuda, 13)
+    L, H, D = 8_500_001, 2, 128
+    q = torch.randn(1, L, H, D, generator=gen, device=cuda, dtype=BF).transpose(1, 2)
+    w = torch.rand(D, generator=gen, device=cuda) * 0.4 - 0.2
+    a = torch.rand(L, D // 2, generator=gen, device=cuda) * 100.0
+    f = torch.stack([a.cos(), -a.sin(), a.sin(), a.cos()], -1).unflatten(-1, (2, 2)).contiguous()
+    got, _ = ops.qk_norm_rope(q, None, w, None, f)
+    for rows in (slice(0, 50), slice(L - 50, L)):
+        R.check(got[:, :, rows], *R.norm_rope(q[:, :, rows], w, f[rows], 1e-6))
+
+
+def test_w4_linear_offsets_past_32_bits(cuda):
+    gen = gen_of(cuda, 14)
+    n, k = 300_001, 16384
+    packed, scales = R.random_w4(n, k, gen, cuda)
+    assert packed.numel() > 2 ** 31
+    x = torch.randn(2, k, generator=gen, device=cuda).to(BF)
+    got = ops.w4_linear(x, packed, scales)
+    for cols in (slice(0, 40), slice(n - 40, n)):
+        R.check(got[:, cols], *R.w4_linear(x, packed[cols], scales[cols], None, True, "none"))
