@@ -1138,18 +1138,19 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
         if (w & XS_FREE) mma_commit(&k_empty[s]);
       };
       uint32_t no = 0;
-      // the first word of the next step that has products
+      // the first word of the next step
       auto fetch = [&]() {
-        for (;;) {
-          const uint32_t at = no % XT_RECORDS;
-          int w = rec_ready(no) ? records[2 * at].x : XS_END;
-          w = warp_uniform(w);
-          if (lane == 0) mbar_arrive(&rec_empty[at]);
-          ++no;
-          if (!(w & XS_EMPTY)) return w;
-        }
+        const uint32_t at = no % XT_RECORDS;
+        int w = rec_ready(no) ? records[2 * at].x : XS_END;
+        w = warp_uniform(w);
+        if (lane == 0) mbar_arrive(&rec_empty[at]);
+        ++no;
+        return w;
       };
-      // cur: the step whose P comes next, nxt: the step whose S does (XS_END: none)
+      // cur: the step whose P comes next (XS_END: none), nxt: the step behind it,
+      // whose S does.  One without keys takes its turn with nothing to issue: to
+      // look past it for one with keys would hold back cur's PV, for which the
+      // softmax warps wait, and with them the records that are being looked for.
       int cur = XS_END, nxt = fetch();
       uint32_t step = 0;
       bool ok = true;
@@ -1157,7 +1158,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
       while (((cur & nxt) & XS_END) == 0) {
         // S of the item's next tile goes out behind PV; the first of another
         // item waits for its queries, which must not hold PV back
-        bool s_due = !(nxt & XS_END);
+        bool s_due = !(nxt & (XS_END | XS_EMPTY));
         if (!(cur & XS_END)) {  // the side data of a ring slot are ready after its V
           const bool both = s_due && !(nxt & XS_FIRST);
           ok = wait(&aux_full[(cur >> 8) & 15], (cur >> 12) & 1) && (!both || k_ready(nxt)) && wait(&p_full[t], step & 1);
@@ -1178,8 +1179,8 @@ __global__ void __launch_bounds__(XT_THREADS, 1)
           if (leader) issue_s(nxt);
           __syncwarp();
         }
-        cur = nxt;
-        if (!(cur & XS_END)) nxt = fetch();
+        cur = nxt & XS_EMPTY ? XS_END : nxt;
+        if (!(nxt & XS_END)) nxt = fetch();
       }
     } else {
       // ---------------------------------------- side data of every K/V load

@@ -188,3 +188,29 @@ def test_qk_norm_rope_waves(cuda, B, H, Hk, Lq, Lk, D, dtype):
     qo, ko = ops.qk_norm_rope(q, k, wq, wk, fq, fk)
     R.check(qo, *R.norm_rope(q, wq, fq, 1e-6), "q")
     R.check(ko, *R.norm_rope(k, wk, fk, 1e-6), "k")
+
+
+@pytest.mark.parametrize("shape", [(8, 48, 12, 2000, 40, 64, BF), (8, 40, 5, 2500, 150, 128, FP), (8, 18, 18, 5000, 40, 64, FP),
+                                   (6, 36, 12, 2600, 300, 128, BF)])
+@pytest.mark.parametrize("kind", ["lengths", "queries", "heads"])
+def test_many_items_without_keys(cuda, shape, kind):
+    """Long rows of items that see nothing, between items that do: latents without keys, blocks of queries or heads whose
+    mask leaves none."""
+    B, H, Hk, Lq, Lk, D, dtype = shape
+    # each of a B200's CTAs gets at least sixteen in a row
+    assert takes_tiles(*shape[:6]) and items(H, Hk, Lq, B) >= 16 * 148
+    q, k, v = inputs(cuda, *shape)
+    lengths = mask = None
+    if kind == "lengths":
+        lengths = torch.tensor([Lk, 0, 0, Lk - 1, 0, 0, 0, 5][:B], dtype=torch.int32, device=cuda)
+    elif kind == "queries":
+        mask = torch.ones(1, 1, Lq, Lk, dtype=torch.bool, device=cuda)
+        mask[:, :, 300:] = False
+    else:
+        mask = torch.zeros(B, H, 1, Lk, dtype=torch.bool, device=cuda)
+        mask[::3, ::9, :, ::2] = True
+    got = ops.cross_attention(q, k, v, lengths=lengths, mask=mask)
+    assert ops.device_error() == 0
+    R.check(got, *R.cross_attention(q, k, v, lengths, mask))
+    gone = ~R.keep_mask(B, H, Lq, Lk, lengths, mask, None, cuda).any(-1)
+    assert not got.view(B, Lq, H, D).transpose(1, 2)[gone].any()
