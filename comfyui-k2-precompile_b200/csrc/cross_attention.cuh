@@ -524,8 +524,8 @@ __device__ __forceinline__ uint4 cross_seen(const CrossTileParams& P, int b, int
 // keys gets all of the weight is all that an addend of this size says).
 __device__ __forceinline__ float cross_addend(float raw) {
   constexpr float kPower = 1.7014118346046923e38f;  // 2^127
-  const float over = fabsf(raw) - kPower;
-  return over > 0.0f && over < INFINITY ? copysignf(fmaf(over, 0.55f, kPower * kLog2e), raw) : raw * kLog2e;
+  const float size = fabsf(raw), low = fminf(size, kPower);
+  return copysignf(fmaf(size - low, 0.55f, low * kLog2e), raw);
 }
 
 __device__ __forceinline__ int cross_keys(const CrossParams& p, int b) {
