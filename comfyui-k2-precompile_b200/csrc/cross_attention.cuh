@@ -671,8 +671,10 @@ __device__ __forceinline__ void tmem_st_row(uint32_t taddr, const uint32_t (&r)[
 // the largest has an exponent of exactly 0 whatever its size (XT_LARGEST).  32
 // keys at a time: a lane's own key for the score, its own columns for PV.  Out of
 // line and once per item: a test of every tile's maximum, with S replaced by its
-// rounded product, took 87 to 90 us on 2 x 4050 queries by 154 keys and 105 to
-// 110 on 4096 by 1000 under a regional mask.
+// rounded product, took 2 x 4050 queries by 154 keys from 87 to 90 us and 4096 by
+// 1000 under a regional mask from 105 to 110.  1024 queries of 48/12 heads by 4096
+// keys, every row done again: 22.9 ms, 0.15 without.  (165 cycles a key and row: the
+// other roles' bounded waits last for a warp's 32 rows up to 700,000 keys.)
 template <typename T, int D>
 __device__ __noinline__ void cross_row(const CrossParams& p, int b, int head, int tok) {
   constexpr int C = D / 32;
@@ -694,7 +696,7 @@ __device__ __noinline__ void cross_row(const CrossParams& p, int b, int head, in
       const uint4* qr = reinterpret_cast<const uint4*>(q);
       const uint4* kr = reinterpret_cast<const uint4*>(k + key * p.k_st);
       float dot = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
       for (int i = 0; i < D / 8; ++i) {
         const uint4 x = __ldg(qr + i), y = __ldg(kr + i);
         const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
@@ -718,11 +720,10 @@ __device__ __noinline__ void cross_row(const CrossParams& p, int b, int head, in
     l = fmaf(l, f, e);
 #pragma unroll
     for (int i = 0; i < C; ++i) o[i] *= f;
-    const uint32_t live = __ballot_sync(0xffffffffu, keep);
-#pragma unroll 4
-    for (int j = 0; j < 32; ++j) {
+    // (at scores of this size few weights are not 0)
+    for (uint32_t live = __ballot_sync(0xffffffffu, e != 0.0f); live; live &= live - 1) {
+      const int j = __ffs(live) - 1;
       const float pj = __shfl_sync(0xffffffffu, e, j);
-      if (!((live >> j) & 1u)) continue;
       const uint32_t* vr = reinterpret_cast<const uint32_t*>(v + (k0 + j) * p.v_st);
 #pragma unroll
       for (int i = 0; i < C; i += 2) {
