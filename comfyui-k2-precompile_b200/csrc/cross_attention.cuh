@@ -12,8 +12,11 @@
 // and shows to others).
 //
 // Scores, row maxima, row sums and O are fp32; P is rounded to the type of V,
-// which the matrix product asks for: 2^-9 (bf16) or 2^-12 (fp16) of each
-// probability, as much as the rounding of the output.
+// which the matrix product asks for.  That costs up to 2^-8 (bf16) or 2^-11
+// (fp16) of each probability, as much as the rounding of the output; an fp16 P
+// below 2^-14 is off by up to 2^-25 instead (P is relative to the row's running
+// maximum, or on the tile kernel to a reference up to 2^8 below it).  Row sums
+// are taken of P before the rounding.
 #pragma once
 #include "elem16.cuh"
 
@@ -47,8 +50,8 @@ struct CrossParams {
 // with byte permutes.
 //
 // Bound by latency: a warp's turn of 16 keys is one trip to memory, products
-// and a join.  Measured: 1 query of 48/12 heads by 4096 keys (25 MB) 13.1 us;
-// 16 queries of 20 heads of 64 by 729 keys, four latents, 10.0.
+// and a join.  Measured: 1 query of 48/12 heads by 4096 keys (25 MB) 11.8 us;
+// 16 queries of 20 heads of 64 by 729 keys, four latents, 9.6.
 constexpr int XF_THREADS = 256;
 constexpr int XF_WARPS = XF_THREADS / 32;
 constexpr int XF_ROWS = 16;
@@ -388,10 +391,12 @@ __global__ void __launch_bounds__(XF_THREADS, D == 64 ? xf_per_sm(64) : 0) cross
 //
 // Bound by the chain S -> softmax -> PV of a slot (3700 cycles for 128 keys of
 // both slots, 2050 of them products) and, for short prompts, by what an item
-// costs at its end.  Measured: 8 x 4224 queries by 2048 keys, 48/12 heads,
-// 1.78 ms, 955 TFLOP/s; 4096 queries by 1000 keys under a regional mask 105 us;
-// 2 x 4050 queries by 154 and 76 keys with addends 87 us (200 MB).  Part of the
-// exponentials as a polynomial on the FMA pipe measured slower.
+// costs at its end.  Measured: 8 x 4224 queries by 2048 keys, 48/12 heads, 1.65
+// ms, 1030 TFLOP/s (1.84 ms, 925, once the power limit has lowered the clock);
+// 4096 queries by 1000 keys under a regional mask 103 us; 2 x 4050 queries by 154
+// and 76 keys with addends 88 us (200 MB).  Part of the exponentials as a
+// polynomial on the FMA pipe measured slower.  The code's layout alone is worth
+// 5%: compare builds, not edits.
 constexpr int XT_BM = 128;
 constexpr int XT_BN = 128;
 constexpr int XT_THREADS = 384;

@@ -2,9 +2,11 @@
 // share: conversions of a pair of 16-bit elements, streaming loads, and the
 // warp-level m16n8k16 matrix product.
 //
-// These operators read far more than they compute (a weight or a key is used
-// by 1..16 rows), so the warp-level product is enough to keep up with memory;
-// the shapes with more rows than that run on tcgen05.
+// w4_linear and the few-row attention kernel read far more than they compute (a
+// weight or a key is used by up to 16 rows at a time), so the warp-level product
+// is enough to keep up with memory.  Attention of many queries runs on tcgen05
+// where that takes less time; w4_linear has no such kernel and reads its weight
+// again for every 16 rows.
 #pragma once
 #include <type_traits>
 

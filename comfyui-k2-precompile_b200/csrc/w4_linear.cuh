@@ -15,8 +15,8 @@
 // rotated in fp32, scaled by a power of two per (row, group) that brings the
 // group's largest value into [2^14, 2^15), and rounded to fp16.  The rounding
 // is relative to the value for everything within 2^28 of the group's maximum,
-// so it costs a rotated row 2^-12 (a bf16 rounding would cost 2^-9, as much as
-// the output's), and an unrotated bf16 or fp16 row nothing.
+// so it costs a rotated row up to 2^-11 (a bf16 rounding would cost 2^-8, as much
+// as the output's), and an unrotated bf16 or fp16 row nothing.
 //
 // w4_linear_kernel: a warp takes 16 weight rows (the product's M) and a
 // contiguous range of groups, straight from the checkpoint's layout: lane
